@@ -70,11 +70,16 @@ def _run(cmd: list[str]) -> None:
 EXTRA_FLAGS = {"flash_attn_fwd.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-fno-slp-vectorize"]}
 
 
+# no packed-fp32 VALU instructions (v_pk_add / mul / fma_f32) in any kernel: some of their forms have given
+# wrong results on this part; the compiler forms them by itself from scalar code
+NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+
+
 def _hip_obj(src: Path, headers: list[Path], force: bool) -> Path:
     out = BUILD / (src.stem + ".hip.o")
     if force or _newer(out, [src, *headers, Path(__file__)]):
         _run(["hipcc", f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-c", str(src), "-o", str(out),
-              "-I", str(CSRC / "kernels"), "-Wno-unused-result", "-ffp-contract=fast", *EXTRA_FLAGS.get(src.name, [])])
+              "-I", str(CSRC / "kernels"), "-Wno-unused-result", "-ffp-contract=fast", *NO_PACKED_FP32, *EXTRA_FLAGS.get(src.name, [])])
     return out
 
 
