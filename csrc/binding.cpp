@@ -5,6 +5,7 @@
 // Every entry point validates device, dtype, contiguity and the shape assumptions of its kernel on
 // the host before launching -- a wrong shape must be a Python exception, never a GPU fault.
 #include <torch/extension.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime.h>
 
@@ -60,6 +61,13 @@ int ftc_flash_bwd(const void* q, const void* k, const void* v, const void* o, co
                   long long dkv_row_stride, float scale, int causal, int window, const int* doc_start,
                   const int* doc_end, int kv_valid, const float* rope_cos, const float* rope_sin,
                   const int* rope_pos, hipStream_t stream);
+int ftc_kv4_store(void* data, const void* k, const void* v, const int* start, const int* count, int B, int KV, int D,
+                  int n, int tiles, long long k_bs, long long k_rs, long long v_bs, long long v_rs, int bias, int limit,
+                  hipStream_t stream);
+int ftc_kv4_load(const void* data, void* k, void* v, const int* start, int B, int KV, int D, int n, int tiles,
+                 hipStream_t stream);
+int ftc_kv4_decode(const void* qkv, void* data, const int* lens, void* out, int B, int H, int KV, int D, int tiles,
+                   int max_len, long long q_rs, long long o_rs, float scale, int window, int sinks, hipStream_t stream);
 int ftc_nf4_dequant(const uint8_t* packed, const uint8_t* absmax_q, const float* absmax_scale, float absmax_offset,
                     void* out, long long n, int block, int block2, hipStream_t stream);
 int ftc_nf4_quant(const void* w, uint8_t* packed, float* absmax, long long n, int block, hipStream_t stream);
@@ -562,6 +570,89 @@ at::Tensor decode_attention(const at::Tensor& q, at::Tensor& k_cache, at::Tensor
   return out;
 }
 
+// ---------------- 4-bit KV cache (csrc/kernels/kv4.h) ----------------
+// All tensors on the cache's device; the kernels run on that device's current stream.
+struct Kv4Dims {
+  int B, KV, tiles;
+};
+Kv4Dims need_kv4(const at::Tensor& data, int64_t D) {
+  need(data, at::kByte, "kv4 cache");
+  TORCH_CHECK(D == 64 || D == 128, "kv4: head_dim 64 or 128");
+  TORCH_CHECK(data.dim() == 4 && data.is_contiguous() && data.size(3) == 64 * (D / 2 + D / 16),
+              "kv4: cache must be a contiguous [B, KV, tiles, record] tensor");
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(data.data_ptr()) % 16 == 0, "kv4: cache must be 16-byte aligned");
+  TORCH_CHECK(data.size(0) >= 1 && data.size(1) >= 1 && data.size(2) >= 1 && data.size(2) < (1LL << 26) &&
+                  data.size(0) <= 0x7fffffff && data.size(1) <= 0x7fffffff, "kv4: cache size");
+  return {(int)data.size(0), (int)data.size(1), (int)data.size(2)};
+}
+inline void need_index(const at::Tensor& t, const at::Tensor& data, const char* name) {
+  need(t, at::kInt, name);
+  TORCH_CHECK(t.device() == data.device() && t.dim() == 1 && t.size(0) == data.size(0) && t.is_contiguous(), name,
+              ": int32 [B] on the cache's device");
+}
+
+void kv4_store_(at::Tensor& data, const at::Tensor& k_in, const at::Tensor& v_in, const at::Tensor& start,
+                const c10::optional<at::Tensor>& count, int64_t D) {
+  const Kv4Dims c = need_kv4(data, D);
+  need(k_in, at::kBFloat16, "k");
+  need(v_in, at::kBFloat16, "v");
+  need_index(start, data, "start");
+  if (count.has_value()) need_index(*count, data, "count");
+  at::Tensor k = k_in, v = v_in;
+  c10::DeviceGuard guard(data.device());
+  for (at::Tensor* t : {&k, &v}) {
+    TORCH_CHECK(t->device() == data.device(), "kv4_store: k, v on the cache's device");
+    TORCH_CHECK(t->dim() == 3 && t->size(0) == c.B && t->size(2) == c.KV * D && t->size(1) == k_in.size(1) &&
+                    t->size(1) >= 1 && t->size(1) <= 0x3fffffff,
+                "kv4_store: k, v [B, n, KV*D]");
+    // rows that cannot be read 16 bytes at a time are copied
+    if (t->stride(2) != 1 || reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 ||
+        (t->size(0) > 1 && t->stride(0) % 8) || (t->size(1) > 1 && t->stride(1) % 8))
+      *t = t->clone(at::MemoryFormat::Contiguous);
+  }
+  check(ftc_kv4_store(data.data_ptr(), k.data_ptr(), v.data_ptr(), start.data_ptr<int>(),
+                      count.has_value() ? count->data_ptr<int>() : nullptr, c.B, c.KV, (int)D, (int)k.size(1), c.tiles,
+                      k.stride(0), k.stride(1), v.stride(0), v.stride(1), 0, 0x7fffffff, cur_stream()),
+        "kv4_store");
+}
+
+std::vector<at::Tensor> kv4_load(const at::Tensor& data, const at::Tensor& start, int64_t n, int64_t D) {
+  const Kv4Dims c = need_kv4(data, D);
+  need_index(start, data, "start");
+  TORCH_CHECK(n >= 1 && n <= 0x3fffffff, "kv4_load: n");
+  c10::DeviceGuard guard(data.device());
+  auto k = at::empty({c.B, n, c.KV * D}, data.options().dtype(at::kBFloat16));
+  auto v = at::empty_like(k);
+  check(ftc_kv4_load(data.data_ptr(), k.data_ptr(), v.data_ptr(), start.data_ptr<int>(), c.B, c.KV, (int)D, (int)n,
+                     c.tiles, cur_stream()),
+        "kv4_load");
+  return {k, v};
+}
+
+at::Tensor decode_attention_kv4(const at::Tensor& qkv_in, at::Tensor& data, const at::Tensor& lens, int64_t H,
+                                int64_t KV, int64_t D, int64_t max_len, double scale, int64_t window, int64_t sinks) {
+  const Kv4Dims c = need_kv4(data, D);
+  need(qkv_in, at::kBFloat16, "qkv");
+  need_index(lens, data, "lens");
+  TORCH_CHECK(KV == c.KV && H >= KV && H % KV == 0, "decode_attention_kv4: heads");
+  TORCH_CHECK(qkv_in.device() == data.device() && qkv_in.dim() == 2 && qkv_in.size(0) == c.B &&
+                  qkv_in.size(1) >= (H + 2 * KV) * D,
+              "decode_attention_kv4: qkv [B, >=(H+2KV)*D] on the cache's device");
+  TORCH_CHECK(max_len >= 1 && max_len <= (int64_t)c.tiles * 32, "decode_attention_kv4: max_len outside the cache");
+  TORCH_CHECK(sinks >= 0, "decode_attention_kv4: sinks");
+  c10::DeviceGuard guard(data.device());
+  at::Tensor qkv = qkv_in;
+  if (qkv.stride(1) != 1 || reinterpret_cast<uintptr_t>(qkv.data_ptr()) % 16 || (c.B > 1 && qkv.stride(0) % 8))
+    qkv = qkv.clone(at::MemoryFormat::Contiguous);
+  auto out = at::empty({c.B, H * D}, qkv.options());
+  const int win = (int)std::min<int64_t>(std::max<int64_t>(window, 0), 0x3fffffff);
+  check(ftc_kv4_decode(qkv.data_ptr(), data.data_ptr(), lens.data_ptr<int>(), out.data_ptr(), c.B, (int)H, (int)KV,
+                       (int)D, c.tiles, (int)max_len, qkv.stride(0), out.stride(0), (float)scale, win,
+                       (int)std::min<int64_t>(sinks, 0x3fffffff), cur_stream()),
+        "decode_attention_kv4");
+  return out;
+}
+
 // ---------------- NF4 (QLoRA) ----------------
 std::vector<at::Tensor> nf4_quantize(const at::Tensor& w, int64_t block) {
   need(w, at::kBFloat16, "w");
@@ -766,6 +857,9 @@ PYBIND11_MODULE(_C, m) {
         py::arg("doc_start") = py::none(), py::arg("doc_end") = py::none(), py::arg("kv_valid") = -1,
         py::arg("rope_cos") = py::none(), py::arg("rope_sin") = py::none(), py::arg("rope_pos") = py::none());
   m.def("decode_attention", &decode_attention);
+  m.def("kv4_store_", &kv4_store_);
+  m.def("kv4_load", &kv4_load);
+  m.def("decode_attention_kv4", &decode_attention_kv4);
   m.def("nf4_quantize", &nf4_quantize);
   m.def("nf4_dequantize", &nf4_dequantize);
   m.def("nf4_linear", &nf4_linear);

@@ -1,0 +1,241 @@
+// Rows of K and V quantised to 4 bits as they are written into a cache, and read back (layout and
+// quantisation: kv4.h).
+//
+// One wave = one record (32 tokens of one kv head).  A lane quantises exactly the 16-byte chunks that the
+// layout gives it: for K its token's 8-value runs of every group (the group maximum is shared by the 4 lanes of
+// that token), for V 8 tokens x 8 (4) values (shared by the lanes of the group), so nothing goes through LDS
+// and whole records are written as linear 16-byte stores.  Records that are only partly covered by the call
+// (its first and last, and every single-token append) store token by token; other tokens' bytes stay.
+// Bound: HBM -- 2 bytes read and 0.5625 written per value (and back).
+#include "kv4.h"
+
+using namespace ftc;
+
+namespace {
+
+struct StoreArgs {
+  uint8_t* data;
+  const uint16_t *k, *v;
+  const int *start, *count;
+  long long k_bs, k_rs, v_bs, v_rs;  // batch / row strides in elements
+  int B, KV, n, tiles, span;         // span: records a sequence's rows can touch
+  int bias, limit;                   // rows go to start[b] + bias + i; a start[b] + bias >= limit writes nothing
+};
+
+// 4-lane or 8-lane (lanes differing in the given xor masks) maximum of packed keys, both halves
+DEV_INLINE uint32_t key_max_x(uint32_t k, int m) { return kv4_max2(k, (uint32_t)__shfl_xor((int)k, m, 64)); }
+DEV_INLINE uint32_t key_top(uint32_t k) {
+  const uint32_t a = k & 0xffffu, b = k >> 16;
+  return a > b ? a : b;
+}
+DEV_INLINE uint32_t keys8(const uint4& u) {
+  return kv4_max2(kv4_max2(kv4_keys(u.x), kv4_keys(u.y)), kv4_max2(kv4_keys(u.z), kv4_keys(u.w)));
+}
+
+template <int D>
+__global__ __launch_bounds__(256) void kv4_store_kernel(StoreArgs a) {
+  using L = Kv4<D>;
+  const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+  const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const long long total = (long long)a.B * a.span * a.KV;
+  if (item >= total) return;
+  const int kvh = (int)(item % a.KV);
+  const int sp = (int)(item / a.KV % a.span), b = (int)(item / a.KV / a.span);
+  const long long start = (long long)a.start[b] + a.bias;
+  if (start >= a.limit) return;
+  const int n = a.count ? min(a.n, a.count[b]) : a.n;
+  // first record that the rows touch inside the cache (rows before position 0 are not written)
+  const long long p0 = start > 0 ? start : 0;
+  const long long tile = p0 / KV4_TILE + sp;
+  if (tile >= a.tiles) return;
+  const long long row0 = tile * KV4_TILE - start;  // row index of the record's token 0
+  if (row0 >= n || row0 + KV4_TILE <= 0) return;
+  const bool whole = row0 >= 0 && row0 + KV4_TILE <= n;
+  uint8_t* rec = a.data + (((long long)b * a.KV + kvh) * a.tiles + tile) * L::REC;
+  const uint16_t* kp = a.k + b * a.k_bs + (long long)kvh * D;
+  const uint16_t* vp = a.v + b * a.v_bs + (long long)kvh * D;
+  auto valid = [&](int t) { return row0 + t >= 0 && row0 + t < n; };
+
+  // ---- K: this lane's token of each half, 8 values of every group
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int t = 8 * (r >> 2) + 4 * half + (r & 3);
+    const bool ok = whole || valid(t);
+    uint32_t w[L::NG];
+#pragma unroll
+    for (int j = 0; j < L::NG; ++j) {
+      uint4 u = make_uint4(0, 0, 0, 0);
+      if (ok) u = *reinterpret_cast<const uint4*>(kp + (row0 + t) * a.k_rs + 32 * j + 8 * q);
+      float rinv, f[8];
+      const uint32_t s = kv4_scale(key_top(key_max_x(key_max_x(keys8(u), 16), 32)), &rinv);
+      unpack8(u, f);
+      w[j] = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[j] |= kv4_code(f[e], rinv) << (16 * (e & 1) + 4 * (e >> 1));
+      if (ok && q == j)
+        *reinterpret_cast<uint16_t*>(rec + L::KS + ((r >> 2) * L::NG + j) * 16 + (4 * half + (r & 3)) * 2) = (uint16_t)s;
+    }
+    if (ok) {
+      if constexpr (D == 128)
+        *reinterpret_cast<uint4*>(rec + L::KC + half * 1024 + lane * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+      else
+        *reinterpret_cast<uint2*>(rec + L::KC + lane * 16 + half * 8) = make_uint2(w[0], w[1]);
+    }
+  }
+
+  // ---- V: tokens 8 q + 0..7, NJ values from d = NJ r
+  uint32_t w[L::CH][4], sc[4];
+#pragma unroll
+  for (int p = 0; p < 4; ++p) {
+#pragma unroll
+    for (int c = 0; c < L::CH; ++c) w[c][p] = 0;
+    sc[p] = 0;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const bool ok = whole || valid(8 * q + i);
+    float f[8], rinv;
+    uint32_t key;
+    if constexpr (D == 128) {
+      uint4 u = make_uint4(0, 0, 0, 0);
+      if (ok) u = *reinterpret_cast<const uint4*>(vp + (row0 + 8 * q + i) * a.v_rs + 8 * r);
+      key = keys8(u);
+      unpack8(u, f);
+    } else {
+      uint2 u = make_uint2(0, 0);
+      if (ok) u = *reinterpret_cast<const uint2*>(vp + (row0 + 8 * q + i) * a.v_rs + 4 * r);
+      key = kv4_max2(kv4_keys(u.x), kv4_keys(u.y));
+      f[0] = bf_lo(u.x); f[1] = bf_hi(u.x); f[2] = bf_lo(u.y); f[3] = bf_hi(u.y);
+    }
+    key = key_max_x(key_max_x(key, 1), 2);
+    if constexpr (D == 64) key = key_max_x(key, 4);
+    sc[i >> 1] |= kv4_scale(key_top(key), &rinv) << (16 * (i & 1));
+#pragma unroll
+    for (int e = 0; e < L::NJ; ++e) w[e >> 2][i >> 1] |= kv4_code(f[e], rinv) << (16 * (i & 1) + 4 * (e & 3));
+  }
+  constexpr int LPG = 16 / L::NG;  // lanes r per group
+  if (whole) {
+#pragma unroll
+    for (int c = 0; c < L::CH; ++c)
+      *reinterpret_cast<uint4*>(rec + L::VC + c * 1024 + lane * 16) = make_uint4(w[c][0], w[c][1], w[c][2], w[c][3]);
+    if (r % LPG == 0)
+      *reinterpret_cast<uint4*>(rec + L::VS + (q * L::NG + r / LPG) * 16) = make_uint4(sc[0], sc[1], sc[2], sc[3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (!valid(8 * q + i)) continue;
+#pragma unroll
+      for (int c = 0; c < L::CH; ++c)
+        *reinterpret_cast<uint16_t*>(rec + L::VC + c * 1024 + lane * 16 + 2 * i) = (uint16_t)(w[c][i >> 1] >> (16 * (i & 1)));
+      if (r % LPG == 0)
+        *reinterpret_cast<uint16_t*>(rec + L::VS + (q * L::NG + r / LPG) * 16 + 2 * i) = (uint16_t)(sc[i >> 1] >> (16 * (i & 1)));
+    }
+  }
+}
+
+struct LoadArgs {
+  const uint8_t* data;
+  uint16_t *k, *v;  // [B, n, KV*D] contiguous
+  const int* start;
+  int B, KV, n, tiles, span;
+};
+
+// Values of one record's tokens as bf16 rows (s * c has 12 significant bits: one rounding).  Rows outside the
+// cache are zeros.  Records are counted from the one of position start[b], which may be negative.
+template <int D>
+__global__ __launch_bounds__(256) void kv4_load_kernel(LoadArgs a) {
+  using L = Kv4<D>;
+  const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+  const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const long long total = (long long)a.B * a.span * a.KV;
+  if (item >= total) return;
+  const int kvh = (int)(item % a.KV);
+  const int sp = (int)(item / a.KV % a.span), b = (int)(item / a.KV / a.span);
+  const long long start = a.start[b];
+  const long long tile = (start >= 0 ? start / KV4_TILE : -((-start + KV4_TILE - 1) / KV4_TILE)) + sp;
+  const long long row0 = tile * KV4_TILE - start;
+  if (row0 >= a.n) return;
+  const bool in = tile >= 0 && tile < a.tiles;
+  const uint8_t* rec = a.data + (((long long)b * a.KV + kvh) * a.tiles + (in ? tile : 0)) * L::REC;
+  const long long W = (long long)a.KV * D;
+  uint16_t* kp = a.k + (long long)b * a.n * W + (long long)kvh * D;
+  uint16_t* vp = a.v + (long long)b * a.n * W + (long long)kvh * D;
+  auto valid = [&](int t) { return row0 + t >= 0 && row0 + t < a.n; };
+
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int t = 8 * (r >> 2) + 4 * half + (r & 3);
+    if (!valid(t)) continue;
+    uint32_t w[L::NG];
+#pragma unroll
+    for (int j = 0; j < L::NG; ++j)
+      w[j] = *reinterpret_cast<const uint32_t*>(rec + L::KC + (D == 128 ? half * 1024 + lane * 16 : lane * 16 + half * 8) + 4 * j);
+#pragma unroll
+    for (int j = 0; j < L::NG; ++j) {
+      const float s = bf2f(*reinterpret_cast<const uint16_t*>(rec + L::KS + ((r >> 2) * L::NG + j) * 16 + (4 * half + (r & 3)) * 2));
+      float f[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = s * ((float)(int)((w[j] >> (16 * (e & 1) + 4 * (e >> 1))) & 15u) - 8.0f);
+      const uint4 u = in ? pack8(f) : make_uint4(0, 0, 0, 0);
+      *reinterpret_cast<uint4*>(kp + (row0 + t) * W + 32 * j + 8 * q) = u;
+    }
+  }
+  constexpr int LPG = 16 / L::NG;
+  uint4 w[L::CH];
+#pragma unroll
+  for (int c = 0; c < L::CH; ++c) w[c] = *reinterpret_cast<const uint4*>(rec + L::VC + c * 1024 + lane * 16);
+  const uint4 sc = *reinterpret_cast<const uint4*>(rec + L::VS + (q * L::NG + r / LPG) * 16);
+  float s[8];
+  unpack8(sc, s);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (!valid(8 * q + i)) continue;
+    float f[8];
+#pragma unroll
+    for (int e = 0; e < L::NJ; ++e) {
+      const uint4& u = w[e >> 2];
+      const uint32_t x = (i >> 1) == 0 ? u.x : (i >> 1) == 1 ? u.y : (i >> 1) == 2 ? u.z : u.w;
+      f[e] = s[i] * ((float)(int)((x >> (16 * (i & 1) + 4 * (e & 3))) & 15u) - 8.0f);
+    }
+    uint16_t* p = vp + (row0 + 8 * q + i) * W + L::NJ * r;
+    if constexpr (D == 128)
+      *reinterpret_cast<uint4*>(p) = in ? pack8(f) : make_uint4(0, 0, 0, 0);
+    else
+      *reinterpret_cast<uint2*>(p) = in ? make_uint2(pack_bf2(f[0], f[1]), pack_bf2(f[2], f[3])) : make_uint2(0, 0);
+  }
+}
+
+}  // namespace
+
+// records that n consecutive positions can touch, wherever they start
+static int kv4_span(int n) { return (n + KV4_TILE - 2) / KV4_TILE + 1; }
+
+extern "C" int ftc_kv4_store(void* data, const void* k, const void* v, const int* start, const int* count, int B, int KV,
+                             int D, int n, int tiles, long long k_bs, long long k_rs, long long v_bs, long long v_rs,
+                             int bias, int limit, hipStream_t stream) {
+  if ((D != 64 && D != 128) || B < 1 || KV < 1 || n < 1 || tiles < 1) return -1;
+  const int span = kv4_span(n);
+  const long long blocks = ((long long)B * KV * span + 3) / 4;
+  if (blocks > 0x7fffffffLL) return -1;
+  StoreArgs a{(uint8_t*)data, (const uint16_t*)k, (const uint16_t*)v, start, count, k_bs, k_rs, v_bs, v_rs,
+              B, KV, n, tiles, span, bias, limit};
+  if (D == 128)
+    hipLaunchKernelGGL(kv4_store_kernel<128>, dim3((unsigned)blocks), dim3(256), 0, stream, a);
+  else
+    hipLaunchKernelGGL(kv4_store_kernel<64>, dim3((unsigned)blocks), dim3(256), 0, stream, a);
+  return (int)hipGetLastError();
+}
+
+extern "C" int ftc_kv4_load(const void* data, void* k, void* v, const int* start, int B, int KV, int D, int n, int tiles,
+                            hipStream_t stream) {
+  if ((D != 64 && D != 128) || B < 1 || KV < 1 || n < 1 || tiles < 1) return -1;
+  const int span = kv4_span(n);
+  const long long blocks = ((long long)B * KV * span + 3) / 4;
+  if (blocks > 0x7fffffffLL) return -1;
+  LoadArgs a{(const uint8_t*)data, (uint16_t*)k, (uint16_t*)v, start, B, KV, n, tiles, span};
+  if (D == 128)
+    hipLaunchKernelGGL(kv4_load_kernel<128>, dim3((unsigned)blocks), dim3(256), 0, stream, a);
+  else
+    hipLaunchKernelGGL(kv4_load_kernel<64>, dim3((unsigned)blocks), dim3(256), 0, stream, a);
+  return (int)hipGetLastError();
+}

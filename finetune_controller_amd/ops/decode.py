@@ -17,6 +17,17 @@ import torch
 from ._backend import ext, use_hip
 
 
+def visible_keys(n: torch.Tensor, L: int, window: int = 0, sinks: int = 0) -> torch.Tensor:
+    """Positions 0..L-1 that the last token of sequences of ``n`` [B] tokens sees, bool [B, L]: all of them, or
+    with ``window`` > 0 the last ``window`` and the first ``sinks``."""
+    t = torch.arange(L, device=n.device)[None]
+    n = n.long()[:, None]
+    ok = t < n
+    if window and window > 0:
+        ok &= (t >= n - window) | (t < sinks)
+    return ok
+
+
 def decode_attention_reference(q, k_cache, v_cache, lens, H: int, KV: int, D: int, scale: float,
                                window: int = 0) -> torch.Tensor:
     """q [B, >=H*D]; caches [B, Lmax, KV*D]; lens [B] valid keys -> [B, H*D] (fp32 math)."""
