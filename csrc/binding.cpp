@@ -66,8 +66,9 @@ int ftc_kv4_store(void* data, const void* k, const void* v, const int* start, co
                   hipStream_t stream);
 int ftc_kv4_load(const void* data, void* k, void* v, const int* start, int B, int KV, int D, int n, int tiles,
                  hipStream_t stream);
-int ftc_kv4_decode(const void* qkv, void* data, const int* lens, void* out, int B, int H, int KV, int D, int tiles,
-                   int max_len, long long q_rs, long long o_rs, float scale, int window, int sinks, hipStream_t stream);
+long long ftc_kv4_decode_workspace_floats(int B, int H, int KV, int D, int max_len, int window, int sinks);
+int ftc_kv4_decode(const void* qkv, void* data, const int* lens, void* out, float* workspace, int B, int H, int KV, int D,
+                   int tiles, int max_len, long long q_rs, long long o_rs, float scale, int window, int sinks, hipStream_t stream);
 int ftc_nf4_dequant(const uint8_t* packed, const uint8_t* absmax_q, const float* absmax_scale, float absmax_offset,
                     void* out, long long n, int block, int block2, hipStream_t stream);
 int ftc_nf4_quant(const void* w, uint8_t* packed, float* absmax, long long n, int block, hipStream_t stream);
@@ -646,9 +647,12 @@ at::Tensor decode_attention_kv4(const at::Tensor& qkv_in, at::Tensor& data, cons
     qkv = qkv.clone(at::MemoryFormat::Contiguous);
   auto out = at::empty({c.B, H * D}, qkv.options());
   const int win = (int)std::min<int64_t>(std::max<int64_t>(window, 0), 0x3fffffff);
-  check(ftc_kv4_decode(qkv.data_ptr(), data.data_ptr(), lens.data_ptr<int>(), out.data_ptr(), c.B, (int)H, (int)KV,
-                       (int)D, c.tiles, (int)max_len, qkv.stride(0), out.stride(0), (float)scale, win,
-                       (int)std::min<int64_t>(sinks, 0x3fffffff), cur_stream()),
+  const int snk = (int)std::min<int64_t>(sinks, 0x3fffffff);
+  auto ws = at::empty({ftc_kv4_decode_workspace_floats(c.B, (int)H, (int)KV, (int)D, (int)max_len, win, snk)},
+                      qkv.options().dtype(at::kFloat));
+  check(ftc_kv4_decode(qkv.data_ptr(), data.data_ptr(), lens.data_ptr<int>(), out.data_ptr(), ws.data_ptr<float>(), c.B,
+                       (int)H, (int)KV, (int)D, c.tiles, (int)max_len, qkv.stride(0), out.stride(0), (float)scale, win, snk,
+                       cur_stream()),
         "decode_attention_kv4");
   return out;
 }
