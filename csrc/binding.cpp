@@ -62,8 +62,7 @@ int ftc_flash_bwd(const void* q, const void* k, const void* v, const void* o, co
                   const int* doc_end, int kv_valid, const float* rope_cos, const float* rope_sin,
                   const int* rope_pos, hipStream_t stream);
 int ftc_kv4_store(void* data, const void* k, const void* v, const int* start, const int* count, int B, int KV, int D,
-                  int n, int tiles, long long k_bs, long long k_rs, long long v_bs, long long v_rs, int bias, int limit,
-                  hipStream_t stream);
+                  int n, int tiles, long long k_bs, long long k_rs, long long v_bs, long long v_rs, hipStream_t stream);
 int ftc_kv4_load(const void* data, void* k, void* v, const int* start, int B, int KV, int D, int n, int tiles,
                  hipStream_t stream);
 long long ftc_kv4_decode_workspace_floats(int B, int H, int KV, int D, int max_len, int window, int sinks);
@@ -572,87 +571,102 @@ at::Tensor decode_attention(const at::Tensor& q, at::Tensor& k_cache, at::Tensor
 }
 
 // ---------------- 4-bit KV cache (csrc/kernels/kv4.h) ----------------
-// All tensors on the cache's device; the kernels run on that device's current stream.
+// Every check of the arguments is here (ops/kv4.py makes the same ones for its torch path); a bad argument is a
+// ValueError.  All tensors are on the cache's device and the kernels run on that device's current stream.
+template <typename... A>
+inline void need_value(bool ok, const A&... msg) {
+  if (!ok) throw pybind11::value_error(c10::str(msg...));
+}
 struct Kv4Dims {
   int B, KV, tiles;
 };
 Kv4Dims need_kv4(const at::Tensor& data, int64_t D) {
-  need(data, at::kByte, "kv4 cache");
-  TORCH_CHECK(D == 64 || D == 128, "kv4: head_dim 64 or 128");
-  TORCH_CHECK(data.dim() == 4 && data.is_contiguous() && data.size(3) == 64 * (D / 2 + D / 16),
-              "kv4: cache must be a contiguous [B, KV, tiles, record] tensor");
-  TORCH_CHECK(reinterpret_cast<uintptr_t>(data.data_ptr()) % 16 == 0, "kv4: cache must be 16-byte aligned");
-  TORCH_CHECK(data.size(0) >= 1 && data.size(1) >= 1 && data.size(2) >= 1 && data.size(2) < (1LL << 26) &&
-                  data.size(0) <= 0x7fffffff && data.size(1) <= 0x7fffffff, "kv4: cache size");
+  need_value(D == 64 || D == 128, "4-bit KV cache: head_dim must be 64 or 128, got ", D);
+  need_value(data.is_cuda() && data.scalar_type() == at::kByte && data.dim() == 4 && data.is_contiguous() &&
+                 data.size(3) == 64 * (D / 2 + D / 16),
+             "4-bit KV cache: expected a contiguous uint8 [B, KV, tiles, ", 64 * (D / 2 + D / 16),
+             "] GPU tensor (kv4_alloc), got ", data.scalar_type(), " ", data.sizes(), " on ", data.device());
+  need_value(data.size(0) >= 1 && data.size(1) >= 1 && data.size(2) >= 1 && data.size(0) < (1LL << 30) &&
+                 data.size(1) < (1LL << 30) && data.size(2) < (1LL << 26) &&
+                 reinterpret_cast<uintptr_t>(data.data_ptr()) % 16 == 0,
+             "4-bit KV cache: size or alignment");
   return {(int)data.size(0), (int)data.size(1), (int)data.size(2)};
 }
 inline void need_index(const at::Tensor& t, const at::Tensor& data, const char* name) {
-  need(t, at::kInt, name);
-  TORCH_CHECK(t.device() == data.device() && t.dim() == 1 && t.size(0) == data.size(0) && t.is_contiguous(), name,
-              ": int32 [B] on the cache's device");
+  need_value(t.scalar_type() == at::kInt && t.device() == data.device() && t.dim() == 1 && t.size(0) == data.size(0) &&
+                 t.is_contiguous(),
+             name, ": int32 [", data.size(0), "] on the cache's device, got ", t.scalar_type(), " ", t.sizes(), " on ",
+             t.device());
+}
+// rows that cannot be read 16 bytes at a time are copied
+inline at::Tensor rows16(const at::Tensor& t) {
+  bool ok = t.stride(-1) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  for (int64_t i = 0; i + 1 < t.dim(); ++i) ok = ok && (t.size(i) <= 1 || t.stride(i) % 8 == 0);
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 
 void kv4_store_(at::Tensor& data, const at::Tensor& k_in, const at::Tensor& v_in, const at::Tensor& start,
-                const c10::optional<at::Tensor>& count, int64_t D) {
+                const c10::optional<at::Tensor>& count) {
+  need_value(k_in.dim() == 3 && k_in.sizes() == v_in.sizes() && k_in.scalar_type() == at::kBFloat16 &&
+                 v_in.scalar_type() == at::kBFloat16 && k_in.device() == data.device() && v_in.device() == data.device(),
+             "kv4_store: k and v must be [B, n, KV*D] of one dtype on the cache's device, got ", k_in.scalar_type(), " ",
+             k_in.sizes(), " and ", v_in.scalar_type(), " ", v_in.sizes());
+  const int64_t KV = data.dim() == 4 ? data.size(1) : 0;
+  need_value(KV > 0 && k_in.size(2) % KV == 0, "kv4_store: ", k_in.size(2), " columns for a cache of ", KV, " kv heads");
+  const int64_t D = k_in.size(2) / KV;
   const Kv4Dims c = need_kv4(data, D);
-  need(k_in, at::kBFloat16, "k");
-  need(v_in, at::kBFloat16, "v");
-  need_index(start, data, "start");
-  if (count.has_value()) need_index(*count, data, "count");
-  at::Tensor k = k_in, v = v_in;
+  need_value(k_in.size(0) == c.B, "kv4_store: ", k_in.size(0), " sequences for a cache of ", c.B);
+  need_index(start, data, "kv4_store: start");
+  if (count.has_value()) need_index(*count, data, "kv4_store: count");
+  const int64_t n = k_in.size(1);
+  need_value(n < (1LL << 30), "kv4_store: too many rows");
+  if (n == 0) return;
   c10::DeviceGuard guard(data.device());
-  for (at::Tensor* t : {&k, &v}) {
-    TORCH_CHECK(t->device() == data.device(), "kv4_store: k, v on the cache's device");
-    TORCH_CHECK(t->dim() == 3 && t->size(0) == c.B && t->size(2) == c.KV * D && t->size(1) == k_in.size(1) &&
-                    t->size(1) >= 1 && t->size(1) <= 0x3fffffff,
-                "kv4_store: k, v [B, n, KV*D]");
-    // rows that cannot be read 16 bytes at a time are copied
-    if (t->stride(2) != 1 || reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 ||
-        (t->size(0) > 1 && t->stride(0) % 8) || (t->size(1) > 1 && t->stride(1) % 8))
-      *t = t->clone(at::MemoryFormat::Contiguous);
-  }
+  const at::Tensor k = rows16(k_in), v = rows16(v_in);
   check(ftc_kv4_store(data.data_ptr(), k.data_ptr(), v.data_ptr(), start.data_ptr<int>(),
-                      count.has_value() ? count->data_ptr<int>() : nullptr, c.B, c.KV, (int)D, (int)k.size(1), c.tiles,
-                      k.stride(0), k.stride(1), v.stride(0), v.stride(1), 0, 0x7fffffff, cur_stream()),
+                      count.has_value() ? count->data_ptr<int>() : nullptr, c.B, c.KV, (int)D, (int)n, c.tiles,
+                      k.stride(0), k.stride(1), v.stride(0), v.stride(1), cur_stream()),
         "kv4_store");
 }
 
-std::vector<at::Tensor> kv4_load(const at::Tensor& data, const at::Tensor& start, int64_t n, int64_t D) {
+std::tuple<at::Tensor, at::Tensor> kv4_load(const at::Tensor& data, const at::Tensor& start, int64_t n, int64_t D) {
   const Kv4Dims c = need_kv4(data, D);
-  need_index(start, data, "start");
-  TORCH_CHECK(n >= 1 && n <= 0x3fffffff, "kv4_load: n");
+  need_index(start, data, "kv4_load: start");
+  need_value(n >= 0 && n < (1LL << 30), "kv4_load: n must not be negative, got ", n);
   c10::DeviceGuard guard(data.device());
   auto k = at::empty({c.B, n, c.KV * D}, data.options().dtype(at::kBFloat16));
   auto v = at::empty_like(k);
-  check(ftc_kv4_load(data.data_ptr(), k.data_ptr(), v.data_ptr(), start.data_ptr<int>(), c.B, c.KV, (int)D, (int)n,
-                     c.tiles, cur_stream()),
-        "kv4_load");
+  if (n > 0)
+    check(ftc_kv4_load(data.data_ptr(), k.data_ptr(), v.data_ptr(), start.data_ptr<int>(), c.B, c.KV, (int)D, (int)n,
+                       c.tiles, cur_stream()),
+          "kv4_load");
   return {k, v};
 }
 
-at::Tensor decode_attention_kv4(const at::Tensor& qkv_in, at::Tensor& data, const at::Tensor& lens, int64_t H,
-                                int64_t KV, int64_t D, int64_t max_len, double scale, int64_t window, int64_t sinks) {
+at::Tensor decode_attention_kv4(const at::Tensor& qkv_in, at::Tensor& data, const at::Tensor& lens, int64_t max_len,
+                                int64_t H, int64_t KV, int64_t D, double scale, int64_t window, int64_t sinks) {
   const Kv4Dims c = need_kv4(data, D);
-  need(qkv_in, at::kBFloat16, "qkv");
-  need_index(lens, data, "lens");
-  TORCH_CHECK(KV == c.KV && H >= KV && H % KV == 0, "decode_attention_kv4: heads");
-  TORCH_CHECK(qkv_in.device() == data.device() && qkv_in.dim() == 2 && qkv_in.size(0) == c.B &&
-                  qkv_in.size(1) >= (H + 2 * KV) * D,
-              "decode_attention_kv4: qkv [B, >=(H+2KV)*D] on the cache's device");
-  TORCH_CHECK(max_len >= 1 && max_len <= (int64_t)c.tiles * 32, "decode_attention_kv4: max_len outside the cache");
-  TORCH_CHECK(sinks >= 0, "decode_attention_kv4: sinks");
+  need_value(KV == c.KV && H >= KV && H % KV == 0 && H < (1LL << 30), "decode_attention_kv4: ", H, " query / ", KV,
+             " kv heads on a cache of ", c.KV);
+  need_value(qkv_in.scalar_type() == at::kBFloat16 && qkv_in.device() == data.device() && qkv_in.dim() == 2 &&
+                 qkv_in.size(0) == c.B && qkv_in.size(1) >= (H + 2 * KV) * D,
+             "decode_attention_kv4: qkv must be [", c.B, ", >=", (H + 2 * KV) * D, "] on the cache's device, got ",
+             qkv_in.sizes(), " on ", qkv_in.device());
+  need_index(lens, data, "decode_attention_kv4: lens");
+  need_value(max_len >= 1 && max_len <= (int64_t)c.tiles * 32, "decode_attention_kv4: max_len ", max_len,
+             " outside the cache's 1..", (int64_t)c.tiles * 32);
+  need_value(sinks >= 0, "decode_attention_kv4: sinks must not be negative, got ", sinks);
   c10::DeviceGuard guard(data.device());
-  at::Tensor qkv = qkv_in;
-  if (qkv.stride(1) != 1 || reinterpret_cast<uintptr_t>(qkv.data_ptr()) % 16 || (c.B > 1 && qkv.stride(0) % 8))
-    qkv = qkv.clone(at::MemoryFormat::Contiguous);
+  const at::Tensor qkv = rows16(qkv_in);
   auto out = at::empty({c.B, H * D}, qkv.options());
-  const int win = (int)std::min<int64_t>(std::max<int64_t>(window, 0), 0x3fffffff);
-  const int snk = (int)std::min<int64_t>(sinks, 0x3fffffff);
-  auto ws = at::empty({ftc_kv4_decode_workspace_floats(c.B, (int)H, (int)KV, (int)D, (int)max_len, win, snk)},
-                      qkv.options().dtype(at::kFloat));
-  check(ftc_kv4_decode(qkv.data_ptr(), data.data_ptr(), lens.data_ptr<int>(), out.data_ptr(), ws.data_ptr<float>(), c.B,
-                       (int)H, (int)KV, (int)D, c.tiles, (int)max_len, qkv.stride(0), out.stride(0), (float)scale, win, snk,
-                       cur_stream()),
+  const int win = (int)std::min<int64_t>(std::max<int64_t>(window, 0), 1 << 30);
+  const int snk = (int)std::min<int64_t>(sinks, 1 << 30);
+  const int64_t wsf = ftc_kv4_decode_workspace_floats(c.B, (int)H, (int)KV, (int)D, (int)max_len, win, snk);
+  at::Tensor ws;
+  if (wsf > 0) ws = at::empty({wsf}, qkv.options().dtype(at::kFloat));
+  check(ftc_kv4_decode(qkv.data_ptr(), data.data_ptr(), lens.data_ptr<int>(), out.data_ptr(),
+                       wsf > 0 ? ws.data_ptr<float>() : nullptr, c.B, (int)H, (int)KV, (int)D, c.tiles, (int)max_len,
+                       qkv.stride(0), out.stride(0), (float)scale, win, snk, cur_stream()),
         "decode_attention_kv4");
   return out;
 }

@@ -74,4 +74,50 @@ DEV_INLINE uint32_t kv4_code(float x, float rinv) {
   return n < 15u ? n : 15u;
 }
 
+// ---- one token's row, quantised by one wave: lanes 0..31 hold K, 32..63 V, 4 values from d = 4 (lane & 31) each
+// (D = 64: the first 16 of each half).  A group of 32 is 8 lanes: its maximum takes two quad permutes and a
+// mirror of 8.
+DEV_INLINE uint32_t kv4_dpp(uint32_t v, int ctrl_is) {
+  return ctrl_is == 1   ? (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xf, 0xf, true)   // lane ^ 1
+         : ctrl_is == 2 ? (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xf, 0xf, true)   // lane ^ 2
+                        : (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xf, 0xf, true);  // 7 - lane of 8
+}
+struct Kv4Token {
+  uint32_t code;   // K: the whole word of the lane pair's 8 values (both lanes); V: 4 nibbles, natural order
+  uint32_t scale;  // bf16 bits of the lane's group
+};
+DEV_INLINE Kv4Token kv4_token(uint2 u, int lane) {
+  uint32_t k2 = kv4_max2(kv4_keys(u.x), kv4_keys(u.y));
+  k2 = kv4_max2(k2, kv4_dpp(k2, 1));
+  k2 = kv4_max2(k2, kv4_dpp(k2, 2));
+  k2 = kv4_max2(k2, kv4_dpp(k2, 3));
+  const uint32_t a = k2 & 0xffffu, b = k2 >> 16;
+  float rinv;
+  Kv4Token t;
+  t.scale = kv4_scale(a > b ? a : b, &rinv);
+  const uint32_t n0 = kv4_code(bf_lo(u.x), rinv), n1 = kv4_code(bf_hi(u.x), rinv);
+  const uint32_t n2 = kv4_code(bf_lo(u.y), rinv), n3 = kv4_code(bf_hi(u.y), rinv);
+  const uint32_t kw = (n0 | n2 << 4 | n1 << 16 | n3 << 20) << (8 * (lane & 1));
+  t.code = lane < 32 ? (kw | kv4_dpp(kw, 1)) : (n0 | n1 << 4 | n2 << 8 | n3 << 12);
+  return t;
+}
+template <int D>
+DEV_INLINE void kv4_put_token(uint8_t* rec, int t, const Kv4Token& x, int lane) {
+  using L = Kv4<D>;
+  const int i5 = lane & 31, d = 4 * i5;
+  if (d >= D) return;
+  const int so = ((t >> 3) * L::NG + (d >> 5)) * 16 + (t & 7) * 2;
+  if (lane < 32) {
+    int off, sh, s;
+    L::k_at(t, d & ~7, &off, &sh, &s);
+    if (!(lane & 1)) *reinterpret_cast<uint32_t*>(rec + off) = x.code;
+    if (!(i5 & 7)) *reinterpret_cast<uint16_t*>(rec + L::KS + so) = (uint16_t)x.scale;
+  } else {
+    int off, sh, s;
+    L::v_at(t, d, &off, &sh, &s);
+    *reinterpret_cast<uint16_t*>(rec + off) = (uint16_t)x.code;
+    if (!(i5 & 7)) *reinterpret_cast<uint16_t*>(rec + L::VS + so) = (uint16_t)x.scale;
+  }
+}
+
 }  // namespace ftc

@@ -19,7 +19,6 @@ struct StoreArgs {
   const int *start, *count;
   long long k_bs, k_rs, v_bs, v_rs;  // batch / row strides in elements
   int B, KV, n, tiles, span;         // span: records a sequence's rows can touch
-  int bias, limit;                   // rows go to start[b] + bias + i; a start[b] + bias >= limit writes nothing
 };
 
 // 4-lane or 8-lane (lanes differing in the given xor masks) maximum of packed keys, both halves
@@ -41,8 +40,7 @@ __global__ __launch_bounds__(256) void kv4_store_kernel(StoreArgs a) {
   if (item >= total) return;
   const int kvh = (int)(item % a.KV);
   const int sp = (int)(item / a.KV % a.span), b = (int)(item / a.KV / a.span);
-  const long long start = (long long)a.start[b] + a.bias;
-  if (start >= a.limit) return;
+  const long long start = a.start[b];
   const int n = a.count ? min(a.n, a.count[b]) : a.n;
   // first record that the rows touch inside the cache (rows before position 0 are not written)
   const long long p0 = start > 0 ? start : 0;
@@ -133,6 +131,25 @@ __global__ __launch_bounds__(256) void kv4_store_kernel(StoreArgs a) {
   }
 }
 
+// Few rows a sequence (a decode step's append): one wave = one token of one kv head, 4 values a lane.  A
+// record's wave would keep 31 of 32 tokens' work idle and its bytewise stores serial.
+template <int D>
+__global__ __launch_bounds__(256) void kv4_store_token_kernel(StoreArgs a) {
+  using L = Kv4<D>;
+  const int lane = threadIdx.x & 63;
+  const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (item >= (long long)a.B * a.n * a.KV) return;
+  const int kvh = (int)(item % a.KV);
+  const int i = (int)(item / a.KV % a.n), b = (int)(item / a.KV / a.n);
+  const int d = (4 * (lane & 31)) % D;
+  const uint16_t* p = (lane < 32 ? a.k + b * a.k_bs + i * a.k_rs : a.v + b * a.v_bs + i * a.v_rs) + (long long)kvh * D + d;
+  const uint2 u = *reinterpret_cast<const uint2*>(p);
+  const long long pos = (long long)a.start[b] + i;
+  if (pos < 0 || pos >= (long long)a.tiles * KV4_TILE || (a.count && i >= a.count[b])) return;
+  kv4_put_token<D>(a.data + (((long long)b * a.KV + kvh) * a.tiles + pos / KV4_TILE) * L::REC, (int)(pos % KV4_TILE),
+                   kv4_token(u, lane), lane);
+}
+
 struct LoadArgs {
   const uint8_t* data;
   uint16_t *k, *v;  // [B, n, KV*D] contiguous
@@ -207,19 +224,27 @@ __global__ __launch_bounds__(256) void kv4_load_kernel(LoadArgs a) {
 
 }  // namespace
 
+// calls of fewer rows go token by token
+constexpr int KV4_STORE_TOKENS = 32;
+
 // records that n consecutive positions can touch, wherever they start
 static int kv4_span(int n) { return (n + KV4_TILE - 2) / KV4_TILE + 1; }
 
 extern "C" int ftc_kv4_store(void* data, const void* k, const void* v, const int* start, const int* count, int B, int KV,
                              int D, int n, int tiles, long long k_bs, long long k_rs, long long v_bs, long long v_rs,
-                             int bias, int limit, hipStream_t stream) {
+                             hipStream_t stream) {
   if ((D != 64 && D != 128) || B < 1 || KV < 1 || n < 1 || tiles < 1) return -1;
   const int span = kv4_span(n);
-  const long long blocks = ((long long)B * KV * span + 3) / 4;
+  const bool tokens = n < KV4_STORE_TOKENS;
+  const long long blocks = ((long long)B * KV * (tokens ? n : span) + 3) / 4;
   if (blocks > 0x7fffffffLL) return -1;
   StoreArgs a{(uint8_t*)data, (const uint16_t*)k, (const uint16_t*)v, start, count, k_bs, k_rs, v_bs, v_rs,
-              B, KV, n, tiles, span, bias, limit};
-  if (D == 128)
+              B, KV, n, tiles, span};
+  if (tokens && D == 128)
+    hipLaunchKernelGGL(kv4_store_token_kernel<128>, dim3((unsigned)blocks), dim3(256), 0, stream, a);
+  else if (tokens)
+    hipLaunchKernelGGL(kv4_store_token_kernel<64>, dim3((unsigned)blocks), dim3(256), 0, stream, a);
+  else if (D == 128)
     hipLaunchKernelGGL(kv4_store_kernel<128>, dim3((unsigned)blocks), dim3(256), 0, stream, a);
   else
     hipLaunchKernelGGL(kv4_store_kernel<64>, dim3((unsigned)blocks), dim3(256), 0, stream, a);

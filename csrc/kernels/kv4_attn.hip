@@ -26,7 +26,8 @@ constexpr float LOG2E = 1.4426950408889634f;
 
 struct Dec4Args {
   const uint16_t* q;
-  const uint8_t* data;
+  const uint16_t *knew, *vnew;  // the current tokens' rows (row stride q_rs)
+  uint8_t* data;
   const int* lens;
   uint16_t* out;
   float* opart;  // [B*H, nsplit, D] unnormalised partial outputs
@@ -37,18 +38,22 @@ struct Dec4Args {
 };
 
 // The visible records of a sequence: sink records [0, ts), then [tl, te); split evenly into parts of `per`
-// records (a multiple of the 4 waves).
+// records (a multiple of the workgroup's NW waves).
 struct Span {
   int len, lo, ts, tl, n, per;
+  bool append;  // the current token is written (a length within max_len)
 };
+template <int NW>
 DEV_INLINE Span span_of(const Dec4Args& a, int b) {
   Span s;
-  s.len = min(a.lens[b], a.max_len);
+  const int len = a.lens[b];
+  s.append = len > 0 && len <= a.max_len;
+  s.len = min(len, a.max_len);
   s.lo = a.window > 0 ? max(0, s.len - a.window) : 0;
   s.tl = s.lo / KV4_TILE;
   s.ts = min((min(a.sinks, s.lo) + KV4_TILE - 1) / KV4_TILE, s.tl);
   s.n = s.len > 0 ? s.ts + (s.len + KV4_TILE - 1) / KV4_TILE - s.tl : 0;
-  s.per = ((s.n + a.nsplit - 1) / a.nsplit + 3) / 4 * 4;
+  s.per = ((s.n + a.nsplit - 1) / a.nsplit + NW - 1) / NW * NW;
   return s;
 }
 
@@ -82,23 +87,65 @@ struct Rec {
   uint4 k[Kv4<D>::CH], v[Kv4<D>::CH], ks, vs;
 };
 template <int D>
-DEV_INLINE void load_rec(Rec<D>& t, const uint8_t* rec, int lane, int so) {
+DEV_INLINE void load_k(Rec<D>& t, const uint8_t* rec, int lane, int so) {
   using L = Kv4<D>;
 #pragma unroll
   for (int c = 0; c < L::CH; ++c) t.k[c] = *reinterpret_cast<const uint4*>(rec + L::KC + c * 1024 + lane * 16);
   t.ks = *reinterpret_cast<const uint4*>(rec + L::KS + so);
+}
+template <int D>
+DEV_INLINE void load_v(Rec<D>& t, const uint8_t* rec, int lane, int so) {
+  using L = Kv4<D>;
 #pragma unroll
   for (int c = 0; c < L::CH; ++c) t.v[c] = *reinterpret_cast<const uint4*>(rec + L::VC + c * 1024 + lane * 16);
   t.vs = *reinterpret_cast<const uint4*>(rec + L::VS + so);
 }
 
+// The current token's codes put into the registers of the wave that read its record (token t of 32): the lanes
+// that hold its chunks take them from the lanes that quantised it, so nothing waits for the store.
+template <int D>
+DEV_INLINE void patch_rec(Rec<D>& x, int t, const Kv4Token& n, int lane) {
+  using L = Kv4<D>;
+  const int r = lane & 15, q = lane >> 4, g = r % L::NG;
+  uint32_t w[L::NG], v[L::CH];
+#pragma unroll
+  for (int j = 0; j < L::NG; ++j) w[j] = __shfl(n.code, 8 * j + 2 * q, 64);
+#pragma unroll
+  for (int c = 0; c < L::CH; ++c) v[c] = __shfl(n.code, 32 + (D == 128 ? 2 * r + c : r), 64);
+  const uint32_t ks = __shfl(n.scale, 8 * g, 64), vs = __shfl(n.scale, 32 + 8 * g, 64);
+  const int half = (t >> 2) & 1;
+  if (r == 4 * (t >> 3) + (t & 3)) {
+    if constexpr (D == 128) {
+      if (half) x.k[1] = make_uint4(w[0], w[1], w[2], w[3]);
+      else x.k[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+      if (half) { x.k[0].z = w[0]; x.k[0].w = w[1]; }
+      else { x.k[0].x = w[0]; x.k[0].y = w[1]; }
+    }
+  }
+  if (q == t >> 3) {
+    const int p = (t & 7) >> 1, sh = 16 * (t & 1);
+    auto put = [&](uint4& u, uint32_t y) __attribute__((always_inline)) {
+      const uint32_t m = 0xffffu << sh, z = y << sh;
+      u.x = p == 0 ? (u.x & ~m) | z : u.x;
+      u.y = p == 1 ? (u.y & ~m) | z : u.y;
+      u.z = p == 2 ? (u.z & ~m) | z : u.z;
+      u.w = p == 3 ? (u.w & ~m) | z : u.w;
+    };
+#pragma unroll
+    for (int c = 0; c < L::CH; ++c) put(x.v[c], v[c]);
+    put(x.ks, ks);
+    put(x.vs, vs);
+  }
+}
+
 // CS sets of 16 columns: HPS = 16 / NG query heads each (4 at D = 128, 8 at D = 64)
-template <int D, int CS>
-__global__ __launch_bounds__(256) void kv4_decode_kernel(Dec4Args a) {
+template <int D, int CS, int NW>
+__global__ __launch_bounds__(64 * NW) void kv4_decode_kernel(Dec4Args a) {
   using L = Kv4<D>;
   constexpr int NG = L::NG, NJ = L::NJ, HPS = 16 / NG;
-  __shared__ float red_m[4][CS][16], red_l[4][CS][16];
-  __shared__ float red_o[4][CS][HPS][D];
+  __shared__ float red_m[NW][CS][16], red_l[NW][CS][16];
+  __shared__ float red_o[NW][CS][HPS][D];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, q = lane >> 4, g = col % NG, hc = col / NG;
@@ -106,9 +153,14 @@ __global__ __launch_bounds__(256) void kv4_decode_kernel(Dec4Args a) {
   const int split = blockIdx.x % a.nsplit, item = blockIdx.x / a.nsplit;
   const int hs = item % nhs, kvh = item / nhs % a.KV, b = item / nhs / a.KV;
   const int h0 = kvh * G + hs * HPS * CS, hn = min(HPS * CS, G - hs * HPS * CS);  // heads of this workgroup
-  const Span sp = span_of(a, b);
+  const Span sp = span_of<NW>(a, b);
   const int v0 = split * sp.per, v1 = min(sp.n, v0 + sp.per);
-  if (v0 >= v1) return;  // the join skips this part too
+  if (v0 >= v1) {  // the join skips this part too
+    if (a.nsplit == 1) {  // an empty sequence
+      for (int e = threadIdx.x; e < hn * D; e += 64 * NW) a.out[(long long)b * a.o_rs + (long long)h0 * D + e] = 0;
+    }
+    return;
+  }
 
   // q of column (h, g): values 32 g + 8 q + 0..7 of its head; zero in the other groups' MFMA steps
   bf16x8 qf[CS][NG];
@@ -138,62 +190,83 @@ __global__ __launch_bounds__(256) void kv4_decode_kernel(Dec4Args a) {
     m[s] = -INFINITY;
     l[s] = 0.f;
   }
-  const uint8_t* base = a.data + ((long long)b * a.KV + kvh) * a.tiles * L::REC;
+  uint8_t* base = a.data + ((long long)b * a.KV + kvh) * a.tiles * L::REC;
   const int so = (q * NG + g) * 16;
   auto tile_of = [&](int v) { return v < sp.ts ? v : v - sp.ts + sp.tl; };
 
-  Rec<D> cur, nxt;
-  int v = v0 + wave;
-  if (v < v1) load_rec<D>(cur, base + (long long)tile_of(v) * L::REC, lane, so);
-  for (; v < v1; v += 4) {
-    const int tile = tile_of(v);
-    if (v + 4 < v1) load_rec<D>(nxt, base + (long long)tile_of(v + 4) * L::REC, lane, so);
-    float ks[8], vs[8];
-    unpack8(cur.ks, ks);
+  // One record in registers; its K is loaded again for the next record as soon as it is used up, its V likewise.
+  // The loads are unconditional (the last record is read once more): under a condition the compiler sinks them to
+  // their use, which cost 294 instead of 193 us at 64 x 16384 tokens (32 / 8 heads x 128); two records in
+  // registers spill their way to 594.
+  Rec<D> cur;
+  {
+    const uint8_t* rec = base + (long long)tile_of(min(v0 + wave, v1 - 1)) * L::REC;
+    load_k<D>(cur, rec, lane, so);
+    load_v<D>(cur, rec, lane, so);
+  }
+  // the wave of the last record quantises the current token, writes it and keeps its codes for that record
+  const bool last = sp.append && v1 == sp.n && (sp.n - 1 - v0) % NW == wave;
+  const int tok = (sp.len - 1) % KV4_TILE;
+  Kv4Token fresh;
+  if (last) {
+    const int d = (4 * (lane & 31)) % D;
+    fresh = kv4_token(*reinterpret_cast<const uint2*>((lane < 32 ? a.knew : a.vnew) + (long long)b * a.q_rs + (long long)kvh * D + d), lane);
+    if (hs == 0) kv4_put_token<D>(base + (long long)((sp.len - 1) / KV4_TILE) * L::REC, tok, fresh, lane);
+  }
+  auto record = [&](int v, bool more) __attribute__((always_inline)) {
+    const int t0 = tile_of(v) * KV4_TILE;
+    const uint8_t* next = base + (long long)tile_of(min(v + NW, v1 - 1)) * L::REC;
+    f32x4 c[CS][2];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+#pragma unroll
+      for (int s = 0; s < CS; ++s) c[s][half] = (f32x4){bias[s], bias[s], bias[s], bias[s]};
+#pragma unroll
+      for (int j = 0; j < NG; ++j) {
+        uint32_t w;
+        if constexpr (D == 128)
+          w = j == 0 ? cur.k[half].x : j == 1 ? cur.k[half].y : j == 2 ? cur.k[half].z : cur.k[half].w;
+        else
+          w = half ? (j ? cur.k[0].w : cur.k[0].z) : (j ? cur.k[0].y : cur.k[0].x);
+        const bf16x8 kf = frag(pair16<0>(w), pair16<1>(w), pair16<2>(w), pair16<3>(w));
+#pragma unroll
+        for (int s = 0; s < CS; ++s) c[s][half] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[s][j], c[s][half], 0, 0, 0);
+      }
+    }
+    float x[CS][8];
+    {
+      float ks[8];
+      unpack8(cur.ks, ks);
+#pragma unroll
+      for (int s = 0; s < CS; ++s)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          x[s][i] = dpp_xor1(c[s][i >> 2][i & 3] * ks[i]);
+          if constexpr (NG == 4) x[s][i] = dpp_xor2(x[s][i]);
+        }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (more) load_k<D>(cur, next, lane, so);
+    __builtin_amdgcn_sched_barrier(0);
+    float vs[8];
     unpack8(cur.vs, vs);
     // tokens outside the length, or before the window and past the sinks: no weight, whatever their bytes hold
-    const int t0 = tile * KV4_TILE;
-    const bool edge = t0 + KV4_TILE > sp.len || (t0 < sp.lo && t0 + KV4_TILE > min(a.sinks, sp.lo));
-    bool ok[8];
-    if (edge) {
+    if (t0 + KV4_TILE > sp.len || (t0 < sp.lo && t0 + KV4_TILE > min(a.sinks, sp.lo))) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int t = t0 + 8 * q + i;
-        ok[i] = t < sp.len && (t >= sp.lo || t < a.sinks);
-        vs[i] = ok[i] ? vs[i] : 0.f;
+        const bool ok = t < sp.len && (t >= sp.lo || t < a.sinks);
+        vs[i] = ok ? vs[i] : 0.f;
+#pragma unroll
+        for (int s = 0; s < CS; ++s) x[s][i] = ok ? x[s][i] : -INFINITY;
       }
     }
     bf16x8 pf[CS];
 #pragma unroll
     for (int s = 0; s < CS; ++s) {
-      f32x4 c[2];
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        c[half] = (f32x4){bias[s], bias[s], bias[s], bias[s]};
-        uint32_t w[NG];
-        if constexpr (D == 128) {
-          w[0] = cur.k[half].x; w[1] = cur.k[half].y; w[2] = cur.k[half].z; w[3] = cur.k[half].w;
-        } else {
-          w[0] = half ? cur.k[0].z : cur.k[0].x;
-          w[1] = half ? cur.k[0].w : cur.k[0].y;
-        }
-#pragma unroll
-        for (int j = 0; j < NG; ++j)
-          c[half] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(frag(pair16<0>(w[j]), pair16<1>(w[j]), pair16<2>(w[j]), pair16<3>(w[j])),
-                                                            qf[s][j], c[half], 0, 0, 0);
-      }
-      float x[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        x[i] = dpp_xor1(c[i >> 2][i & 3] * ks[i]);
-        if constexpr (NG == 4) x[i] = dpp_xor2(x[i]);
-        x[i] *= a.c;
-      }
-      if (edge) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = ok[i] ? x[i] : -INFINITY;
-      }
-      float mt = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+      // c > 0: the maximum commutes with the scale
+      float mt = fmaxf(fmaxf(fmaxf(x[s][0], x[s][1]), fmaxf(x[s][2], x[s][3])),
+                       fmaxf(fmaxf(x[s][4], x[s][5]), fmaxf(x[s][6], x[s][7]))) * a.c;
       if (__builtin_amdgcn_ballot_w64(mt > m[s] + 8.0f) != 0) {
         const float mn = fmaxf(m[s], max_q(mt));
         const float al = __builtin_amdgcn_exp2f(m[s] - (mn == -INFINITY ? 0.f : mn));
@@ -207,33 +280,40 @@ __global__ __launch_bounds__(256) void kv4_decode_kernel(Dec4Args a) {
         for (int i = 0; i < 4; ++i) accs[s][i] *= al;
       }
       const float mref = m[s] == -INFINITY ? 0.f : m[s];
-      float p[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        p[i] = __builtin_amdgcn_exp2f(x[i] - mref);
-        l[s] += p[i];
-        p[i] *= vs[i];
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[s][i], a.c, -mref));
+        l[s] += p;
+        x[s][i] = p * vs[i];
       }
-      pf[s] = frag(pack_bf2(p[0], p[1]), pack_bf2(p[2], p[3]), pack_bf2(p[4], p[5]), pack_bf2(p[6], p[7]));
+      pf[s] = frag(pack_bf2(x[s][0], x[s][1]), pack_bf2(x[s][2], x[s][3]), pack_bf2(x[s][4], x[s][5]), pack_bf2(x[s][6], x[s][7]));
       accs[s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, pf[s], accs[s], 0, 0, 0);
     }
+    auto pv = [&](int jj, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) __attribute__((always_inline)) {
+#pragma unroll
+      for (int s = 0; s < CS; ++s)
+        acc[s][jj] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(frag(a0, a1, a2, a3), pf[s], acc[s][jj], 0, 0, 0);
+    };
 #pragma unroll
     for (int c = 0; c < L::CH; ++c) {
       const uint4 w = cur.v[c];
-      const bf16x8 vf[4] = {frag(pair16<0>(w.x), pair16<0>(w.y), pair16<0>(w.z), pair16<0>(w.w)),
-                            frag(pair16<1>(w.x), pair16<1>(w.y), pair16<1>(w.z), pair16<1>(w.w)),
-                            frag(pair16<2>(w.x), pair16<2>(w.y), pair16<2>(w.z), pair16<2>(w.w)),
-                            frag(pair16<3>(w.x), pair16<3>(w.y), pair16<3>(w.z), pair16<3>(w.w))};
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int s = 0; s < CS; ++s)
-          acc[s][4 * c + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[i], pf[s], acc[s][4 * c + i], 0, 0, 0);
+      pv(4 * c + 0, pair16<0>(w.x), pair16<0>(w.y), pair16<0>(w.z), pair16<0>(w.w));
+      pv(4 * c + 1, pair16<1>(w.x), pair16<1>(w.y), pair16<1>(w.z), pair16<1>(w.w));
+      pv(4 * c + 2, pair16<2>(w.x), pair16<2>(w.y), pair16<2>(w.z), pair16<2>(w.w));
+      pv(4 * c + 3, pair16<3>(w.x), pair16<3>(w.y), pair16<3>(w.z), pair16<3>(w.w));
     }
-    cur = nxt;
+    __builtin_amdgcn_sched_barrier(0);
+    if (more) load_v<D>(cur, next, lane, so);
+  };
+  // the current token's record is peeled off: patching it inside the loop makes every record's loads wait
+  int v = v0 + wave;
+  for (const int ve = last ? v1 - 1 : v1; v < ve; v += NW) record(v, true);
+  if (last) {
+    patch_rec<D>(cur, tok, fresh, lane);
+    record(v, false);
   }
 
-  // ---- join the four waves: common maximum per column, then the sums
+  // ---- join the waves: common maximum per column, then the sums in wave order
 #pragma unroll
   for (int s = 0; s < CS; ++s) {
     l[s] = sum_q(l[s]);
@@ -241,11 +321,12 @@ __global__ __launch_bounds__(256) void kv4_decode_kernel(Dec4Args a) {
   }
   __syncthreads();
   const bool mine = g == (NG == 4 ? q : q >> 1);  // this lane's rows (d) are in its column's group
-  float M[CS];
 #pragma unroll
   for (int s = 0; s < CS; ++s) {
-    M[s] = fmaxf(fmaxf(red_m[0][s][col], red_m[1][s][col]), fmaxf(red_m[2][s][col], red_m[3][s][col]));
-    const float al = __builtin_amdgcn_exp2f(m[s] - (M[s] == -INFINITY ? 0.f : M[s]));
+    float M = red_m[0][s][col];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) M = fmaxf(M, red_m[w][s][col]);
+    const float al = __builtin_amdgcn_exp2f(m[s] - (M == -INFINITY ? 0.f : M));
     if (q == 0) red_l[wave][s][col] = l[s] * al;
     if (mine) {
 #pragma unroll
@@ -255,65 +336,122 @@ __global__ __launch_bounds__(256) void kv4_decode_kernel(Dec4Args a) {
     }
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < hn * D; e += 256) {
-    const int h = e / D, d = e % D, s = h / HPS, c = (h % HPS);
-    float o = 0.f;
+  for (int e = threadIdx.x; e < hn * D; e += 64 * NW) {
+    const int h = e / D, d = e % D, s = h / HPS, c = (h % HPS) * NG;
+    float o = 0.f, lt = 0.f, M = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) o += red_o[w][s][c][d];
-    const long long row = ((long long)b * a.H + h0 + h) * a.nsplit + split;
-    a.opart[row * D + d] = o;
-    if (d == 0) {
-      a.ml[row * 2] = fmaxf(fmaxf(red_m[0][s][c * NG], red_m[1][s][c * NG]), fmaxf(red_m[2][s][c * NG], red_m[3][s][c * NG]));
-      a.ml[row * 2 + 1] = red_l[0][s][c * NG] + red_l[1][s][c * NG] + red_l[2][s][c * NG] + red_l[3][s][c * NG];
+    for (int w = 0; w < NW; ++w) {
+      o += red_o[w][s][h % HPS][d];
+      lt += red_l[w][s][c];
+      M = fmaxf(M, red_m[w][s][c]);
+    }
+    if (a.nsplit == 1) {
+      a.out[(long long)b * a.o_rs + (long long)(h0 + h) * D + d] = f2bf(o / lt);
+    } else {
+      const long long row = ((long long)b * a.H + h0 + h) * a.nsplit + split;
+      a.opart[row * D + d] = o;
+      if (d == 0) {
+        a.ml[row * 2] = M;
+        a.ml[row * 2 + 1] = lt;
+      }
     }
   }
 }
 
-// Partials of a (sequence, head) joined in split order.
-template <int D>
-__global__ __launch_bounds__(D) void kv4_join_kernel(Dec4Args a) {
-  const int bh = blockIdx.x, d = threadIdx.x;
-  const Span sp = span_of(a, bh / a.H);
+// Partials of a (sequence, head) joined: 256 threads = 256 / D groups of parts side by side, summed in a fixed
+// order.
+template <int D, int NW>
+__global__ __launch_bounds__(256) void kv4_join_kernel(Dec4Args a) {
+  constexpr int PG = 256 / D;
+  __shared__ float ol[PG][D], ll[PG];
+  const int bh = blockIdx.x, d = threadIdx.x % D, pg = threadIdx.x / D;
+  const Span sp = span_of<NW>(a, bh / a.H);
   const int parts = sp.n > 0 ? (sp.n + sp.per - 1) / sp.per : 0;
-  const long long base = (long long)bh * a.nsplit;
+  const float* ml = a.ml + (long long)bh * a.nsplit * 2;
+  const float* op = a.opart + (long long)bh * a.nsplit * D + d;
   float M = -INFINITY;
-  for (int s = 0; s < parts; ++s) M = fmaxf(M, a.ml[(base + s) * 2]);
+#pragma unroll 8
+  for (int s = 0; s < parts; ++s) M = fmaxf(M, ml[2 * s]);
+  if (M == -INFINITY) M = 0.f;
   float l = 0.f, o = 0.f;
-  for (int s = 0; s < parts; ++s) {
-    const float w = __builtin_amdgcn_exp2f(a.ml[(base + s) * 2] - (M == -INFINITY ? 0.f : M));
-    l += w * a.ml[(base + s) * 2 + 1];
-    o += w * a.opart[(base + s) * D + d];
+#pragma unroll 8
+  for (int s = pg; s < parts; s += PG) {
+    const float w = __builtin_amdgcn_exp2f(ml[2 * s] - M);
+    l += w * ml[2 * s + 1];
+    o += w * op[(long long)s * D];
   }
-  a.out[(long long)(bh / a.H) * a.o_rs + (long long)(bh % a.H) * D + d] = f2bf(parts > 0 ? o / l : 0.f);
+  ol[pg][d] = o;
+  if (d == 0) ll[pg] = l;
+  __syncthreads();
+  if (pg == 0) {
+#pragma unroll
+    for (int i = 1; i < PG; ++i) {
+      o += ol[i][d];
+      l += ll[i];
+    }
+    a.out[(long long)(bh / a.H) * a.o_rs + (long long)(bh % a.H) * D + d] = f2bf(parts > 0 ? o / l : 0.f);
+  }
 }
 
-// column sets a workgroup takes: enough for the group's query heads, at most 4 (16 heads at D = 128)
-int kv4_sets(int D, int G) {
-  const int hps = D == 128 ? 4 : 8, need = (G + hps - 1) / hps;
-  return need >= 3 ? 4 : need;
-}
-// parts a sequence is split into: ~1024 workgroups (16 waves a CU), each wave at least one record
-int kv4_nsplit(int B, int H, int KV, int D, int max_len, int window, int sinks) {
-  const int G = H / KV, cs = kv4_sets(D, G), hps = D == 128 ? 4 : 8;
-  const long long items = (long long)B * KV * ((G + hps * cs - 1) / (hps * cs));
+// column sets a workgroup takes: enough for the group's query heads, at most 2 (8 heads at D = 128, 16 at 64);
+// larger groups take several workgroups
+int kv4_sets(int D, int G) { return G > (D == 128 ? 4 : 8) ? 2 : 1; }
+struct Plan {
+  int cs, nhs, nw, nsplit;
+};
+Plan kv4_plan(int B, int H, int KV, int D, int max_len, int window, int sinks) {
+  Plan p;
+  const int G = H / KV, hps = D == 128 ? 4 : 8;
+  p.cs = kv4_sets(D, G);
+  p.nhs = (G + hps * p.cs - 1) / (hps * p.cs);
+  const long long items = (long long)B * KV * p.nhs;
   long long vis = (max_len + KV4_TILE - 1) / KV4_TILE;
   if (window > 0) {
     const long long w = ((long long)sinks + KV4_TILE - 1) / KV4_TILE + ((long long)window + KV4_TILE - 1) / KV4_TILE + 1;
     vis = w < vis ? w : vis;
   }
-  long long n = (1024 + items - 1) / items;
-  const long long most = (vis + 3) / 4;
-  return (int)(n < most ? n : most);
+  // 8 waves share an item's records (one workgroup a CU), 4 where there are many short items (64 sequences of 300
+  // tokens, 512 items: 8.9 us with 4 waves, 11.5 with 8).
+  p.nw = items > 256 && vis < 32 ? 4 : 8;
+  // Parts: the number that a model of the launch finds quickest -- rounds of 256 workgroups, 1.8 us a record and
+  // wave (the cache bytes at 5.2 TB/s) plus 2.5 us a workgroup, and 3 us for the join.  Measured against every
+  // split from 1 to 128: it picks the quickest or one within 4 % (one 32768-token sequence, 8 items: 32 parts
+  // 15.0 us, 24 parts 16.4, unsplit 192; 16 sequences at a 4096 window: 2 parts 18.9, 1 part 30.9; 32 x 4096
+  // tokens: unsplit 25.3, 2 parts 30.0).
+  float best = 3e38f;
+  p.nsplit = 1;
+  const long long most = vis / p.nw < 1 ? 1 : (vis + p.nw - 1) / p.nw;
+  for (long long n = 1; n <= most && n <= 256; ++n) {
+    const long long rounds = (items * n + 255) / 256, per = ((vis + n - 1) / n + p.nw - 1) / p.nw;
+    const float us = rounds * (per * 1.8f + 2.5f) + (n > 1 ? 3.f : 0.f);
+    if (us < best) {
+      best = us;
+      p.nsplit = (int)n;
+    }
+  }
+  return p;
+}
+
+template <int D, int CS, int NW>
+void launch(const Dec4Args& a, const Plan& p, hipStream_t stream) {
+  hipLaunchKernelGGL((kv4_decode_kernel<D, CS, NW>), dim3((unsigned)((long long)a.B * a.KV * p.nhs * p.nsplit)), dim3(64 * NW),
+                     0, stream, a);
+  if (p.nsplit > 1)
+    hipLaunchKernelGGL((kv4_join_kernel<D, NW>), dim3((unsigned)(a.B * a.H)), dim3(256), 0, stream, a);
+}
+template <int D>
+void launch_d(const Dec4Args& a, const Plan& p, hipStream_t stream) {
+  if (p.cs == 1)
+    p.nw == 8 ? launch<D, 1, 8>(a, p, stream) : launch<D, 1, 4>(a, p, stream);
+  else
+    p.nw == 8 ? launch<D, 2, 8>(a, p, stream) : launch<D, 2, 4>(a, p, stream);
 }
 
 }  // namespace
 
-extern "C" int ftc_kv4_store(void* data, const void* k, const void* v, const int* start, const int* count, int B, int KV,
-                             int D, int n, int tiles, long long k_bs, long long k_rs, long long v_bs, long long v_rs,
-                             int bias, int limit, hipStream_t stream);
-
 extern "C" long long ftc_kv4_decode_workspace_floats(int B, int H, int KV, int D, int max_len, int window, int sinks) {
-  return (long long)B * H * kv4_nsplit(B, H, KV, D, max_len, window, sinks) * (D + 2);
+  const Plan p = kv4_plan(B, H, KV, D, max_len, window, sinks);
+  return p.nsplit > 1 ? (long long)B * H * p.nsplit * (D + 2) : 0;
 }
 
 extern "C" int ftc_kv4_decode(const void* qkv, void* data, const int* lens, void* out, float* workspace, int B, int H,
@@ -321,25 +459,12 @@ extern "C" int ftc_kv4_decode(const void* qkv, void* data, const int* lens, void
                               int sinks, hipStream_t stream) {
   if ((D != 64 && D != 128) || B < 1 || KV < 1 || H < KV || H % KV || max_len < 1 || max_len > (long long)tiles * KV4_TILE)
     return -1;
-  const int nsplit = kv4_nsplit(B, H, KV, D, max_len, window, sinks), G = H / KV, cs = kv4_sets(D, G), hps = D == 128 ? 4 : 8;
-  const long long blocks = (long long)B * KV * ((G + hps * cs - 1) / (hps * cs)) * nsplit;
-  if (blocks > 0x7fffffffLL || (long long)B * H > 0x7fffffffLL) return -1;
+  const Plan p = kv4_plan(B, H, KV, D, max_len, window, sinks);
+  if ((long long)B * KV * p.nhs * p.nsplit > 0x7fffffffLL || (long long)B * H > 0x7fffffffLL) return -1;
   const uint16_t* qp = (const uint16_t*)qkv;
-  // the new token's row: position lens - 1
-  const int rc = ftc_kv4_store(data, qp + (long long)H * D, qp + (long long)(H + KV) * D, lens, nullptr, B, KV, D, 1,
-                               tiles, q_rs, 0, q_rs, 0, -1, max_len, stream);
-  if (rc) return rc;
-  Dec4Args a{qp, (const uint8_t*)data, lens, (uint16_t*)out, workspace, workspace + (long long)B * H * nsplit * D, q_rs, o_rs,
-             B, H, KV, tiles, max_len, window, sinks, nsplit, scale * LOG2E};
-  const dim3 grid((unsigned)blocks), join((unsigned)(B * H));
-#define KV4_LAUNCH(DD, CC) hipLaunchKernelGGL((kv4_decode_kernel<DD, CC>), grid, dim3(256), 0, stream, a)
-  if (D == 128) {
-    if (cs == 1) KV4_LAUNCH(128, 1); else if (cs == 2) KV4_LAUNCH(128, 2); else KV4_LAUNCH(128, 4);
-    hipLaunchKernelGGL(kv4_join_kernel<128>, join, dim3(128), 0, stream, a);
-  } else {
-    if (cs == 1) KV4_LAUNCH(64, 1); else if (cs == 2) KV4_LAUNCH(64, 2); else KV4_LAUNCH(64, 4);
-    hipLaunchKernelGGL(kv4_join_kernel<64>, join, dim3(64), 0, stream, a);
-  }
-#undef KV4_LAUNCH
+  Dec4Args a{qp, qp + (long long)H * D, qp + (long long)(H + KV) * D, (uint8_t*)data, lens, (uint16_t*)out, workspace,
+             workspace + (long long)B * H * p.nsplit * D, q_rs, o_rs, B, H, KV, tiles, max_len, window, sinks, p.nsplit,
+             scale * LOG2E};
+  D == 128 ? launch_d<128>(a, p, stream) : launch_d<64>(a, p, stream);
   return (int)hipGetLastError();
 }

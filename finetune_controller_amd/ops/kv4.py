@@ -146,6 +146,9 @@ def kv4_store(data: torch.Tensor, k: torch.Tensor, v: torch.Tensor, start: torch
     ``start`` int32 [B].  ``count`` (int32 [B], optional): only the first ``count[b]`` rows of sequence b are
     written (a padded batch).  Rows that fall outside the cache are not written; nothing else of the cache
     changes."""
+    if use_hip(k) and k.dtype == torch.bfloat16:
+        ext().kv4_store_(data, k, v, start, count)
+        return
     if k.dim() != 3 or k.shape != v.shape or k.dtype != v.dtype or k.device != v.device or k.device != data.device:
         raise ValueError(f"kv4_store: k and v must be [B, n, KV*D] of one dtype on the cache's device, got "
                          f"{k.dtype} {tuple(k.shape)} and {v.dtype} {tuple(v.shape)}")
@@ -162,9 +165,6 @@ def kv4_store(data: torch.Tensor, k: torch.Tensor, v: torch.Tensor, start: torch
     n = k.shape[1]
     if n == 0:
         return
-    if use_hip(k) and k.dtype == torch.bfloat16:
-        ext().kv4_store_(data, k, v, start, count, D)
-        return
     i = torch.arange(n, device=data.device)
     pos = start.long()[:, None] + i
     ok = (pos >= 0) & (pos < cap)
@@ -179,12 +179,12 @@ def kv4_load(data: torch.Tensor, start: torch.Tensor, n: int, D: int,
              dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
     """The values of positions ``start[b] + 0 .. n - 1``: K and V rows [B, n, KV*D] in ``dtype`` (positions
     outside the cache give zero rows)."""
+    if use_hip(data) and dtype == torch.bfloat16:
+        return ext().kv4_load(data, start, n, D)
     B, KV, cap = _check_cache(data, D)
     _check_index("kv4_load: start", start, data, B)
     if n < 0:
         raise ValueError(f"kv4_load: n must not be negative, got {n}")
-    if use_hip(data) and dtype == torch.bfloat16 and n > 0:
-        return ext().kv4_load(data, start, n, D)
     pos = start.long()[:, None] + torch.arange(n, device=data.device)
     ok = (pos >= 0) & (pos < cap)
     out = []
@@ -222,6 +222,9 @@ def decode_attention_kv4(qkv: torch.Tensor, data: torch.Tensor, lens: torch.Tens
     ``lens - 1`` and attended to as they are held.  ``lens`` int32 [B] counts the current token; ``max_len``
     (host int) bounds it (a longer sequence is attended to over its first ``max_len`` tokens and not written).  ``window`` > 0: the last ``window`` tokens and the first ``sinks`` are seen.  A
     sequence of length 0 writes nothing and gives a zero row."""
+    scale = scale if scale is not None else 1.0 / math.sqrt(D)
+    if use_hip(qkv) and qkv.dtype == torch.bfloat16:
+        return ext().decode_attention_kv4(qkv, data, lens, max_len, H, KV, D, scale, window or 0, sinks)
     B, nkv, cap = _check_cache(data, D)
     if nkv != KV or KV < 1 or H < KV or H % KV:
         raise ValueError(f"decode_attention_kv4: {H} query / {KV} kv heads on a cache of {nkv}")
@@ -233,10 +236,7 @@ def decode_attention_kv4(qkv: torch.Tensor, data: torch.Tensor, lens: torch.Tens
         raise ValueError(f"decode_attention_kv4: max_len {max_len} outside the cache's 1..{cap}")
     if sinks < 0:
         raise ValueError(f"decode_attention_kv4: sinks must not be negative, got {sinks}")
-    scale = scale if scale is not None else 1.0 / math.sqrt(D)
     window = max(0, int(window or 0))
-    if use_hip(qkv) and qkv.dtype == torch.bfloat16:
-        return ext().decode_attention_kv4(qkv, data, lens, H, KV, D, int(max_len), scale, window, int(sinks))
     new = qkv[:, H * D:(H + 2 * KV) * D].unflatten(1, (2, KV * D))
     kv4_store(data, new[:, None, 0], new[:, None, 1], torch.where(lens <= max_len, lens - 1, lens - lens - 1))
     return decode_attention_kv4_reference(qkv, data, lens.clamp(max=max_len), H, KV, D, scale, window, sinks)

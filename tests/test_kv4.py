@@ -192,14 +192,16 @@ def test_decode_reference(B, H, KV, D, lens, window, sinks):
     _check(got, *_expected(qkv, k, v, lens, H, KV, D, scale, window, sinks))
 
 
-def test_refusals():
-    i32 = dict(dtype=torch.int32)
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_refusals(dev):
+    """The same calls are refused on both paths, before anything is launched or written."""
+    i32 = dict(dtype=torch.int32, device=dev)
     with pytest.raises(ValueError, match="head_dim"):
         ops.kv4_alloc(1, 32, 1, 96)
     with pytest.raises(ValueError, match="positive"):
         ops.kv4_alloc(1, 0, 1, 64)
-    data = ops.kv4_alloc(2, 64, 2, 64)
-    k, z = torch.zeros(2, 3, 128, dtype=BF), torch.zeros(2, **i32)
+    data = ops.kv4_alloc(2, 64, 2, 64, device=dev)
+    k, z = torch.zeros(2, 3, 128, dtype=BF, device=dev), torch.zeros(2, **i32)
     for bad in (dict(k=k[:, :, :127]), dict(k=k[:1]), dict(start=z.long()), dict(start=z[:1]),
                 dict(count=torch.zeros(3, **i32)), dict(data=data.float()), dict(data=data[:, :, ::2]), dict(data=data[0])):
         a = {**dict(data=data, k=k, start=z, count=None), **bad}
@@ -209,13 +211,20 @@ def test_refusals():
         ops.kv4_store(data, k, k.float(), z)
     with pytest.raises(ValueError, match="negative"):
         ops.kv4_load(data, z, -1, 64)
-    q, n = torch.zeros(2, 8 * 64, dtype=BF), torch.ones(2, **i32)
+    q, n = torch.zeros(2, 8 * 64, dtype=BF, device=dev), torch.ones(2, **i32)
     for args in ((q, n, 65, 4, 2), (q, n, 0, 4, 2), (q, n, 64, 5, 2), (q, n, 64, 4, 1), (q[:, :400], n, 64, 4, 2),
                  (q[:1], n, 64, 4, 2), (q, n.long(), 64, 4, 2)):
         with pytest.raises(ValueError):
             ops.decode_attention_kv4(args[0], data, args[1], args[2], args[3], args[4], 64)
     with pytest.raises(ValueError, match="sinks"):
         ops.decode_attention_kv4(q, data, n, 64, 4, 2, 64, window=4, sinks=-1)
+    for bad in (dict(data=data.cpu()), dict(start=z.cpu()), dict(v=k.cpu())):
+        if dev == "cuda":  # tensors of another device
+            a = {**dict(data=data, v=k, start=z), **bad}
+            with pytest.raises(ValueError):
+                ops.kv4_store(a["data"], k, a["v"], a["start"])
+    ops.kv4_store(data, k[:, :0], k[:, :0], z)
+    assert ops.kv4_load(data, z, 0, 64)[0].shape == (2, 0, 128)
     assert int(data.sum()) == 0  # nothing was written
 
 
