@@ -61,6 +61,13 @@ int ftc_flash_bwd(const void* q, const void* k, const void* v, const void* o, co
                   long long dkv_row_stride, float scale, int causal, int window, const int* doc_start,
                   const int* doc_end, int kv_valid, const float* rope_cos, const float* rope_sin,
                   const int* rope_pos, hipStream_t stream);
+int ftc_sink_fwd(const void* q, const void* k, const void* v, void* o, float* lse, int B, int S, int H, int KV, int D,
+                 long long q_rs, long long kv_rs, long long o_rs, float scale, int window, int sinks, hipStream_t stream);
+long long ftc_sink_bwd_workspace(int B, int S, int H, int KV, int D, int window, int sinks);
+int ftc_sink_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, const float* lse, void* dq,
+                 void* dk, void* dv, float* workspace, int B, int S, int H, int KV, int D, long long q_rs, long long kv_rs,
+                 long long o_rs, long long do_rs, long long dq_rs, long long dkv_rs, float scale, int window, int sinks,
+                 const float* rope_cos, const float* rope_sin, const int* rope_pos, hipStream_t stream);
 int ftc_kv4_store(void* data, const void* k, const void* v, const int* start, const int* count, int B, int KV, int D,
                   int n, int tiles, long long k_bs, long long k_rs, long long v_bs, long long v_rs, hipStream_t stream);
 int ftc_kv4_load(const void* data, void* k, void* v, const int* start, int B, int KV, int D, int n, int tiles,
@@ -537,6 +544,89 @@ void flash_bwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, co
         "flash_bwd");
 }
 
+// ---------------- flash attention with a window and sinks (csrc/kernels/flash_sink.hip) ----------------
+// q, k, v are head-column views of one packed [B*S, (H+2KV)*D] projection (16-byte aligned rows), any S.
+inline void need_packed(const at::Tensor& qkv, int64_t B, int64_t S, int64_t W, const char* name) {
+  need(qkv, at::kBFloat16, name);
+  TORCH_CHECK(qkv.dim() == 2 && qkv.size(0) == B * S && qkv.size(1) >= W && qkv.stride(1) == 1 &&
+                  qkv.stride(0) % 8 == 0 && qkv.stride(0) >= W && reinterpret_cast<uintptr_t>(qkv.data_ptr()) % 16 == 0,
+              name, " must be a [", B * S, ", >=", W, "] row view with 16-byte aligned rows");
+}
+inline void need_sink_dims(int64_t B, int64_t S, int64_t H, int64_t KV, int64_t D, int64_t window, int64_t sinks) {
+  TORCH_CHECK(D == 64 || D == 128, "sink attention: head_dim 64 or 128");
+  TORCH_CHECK(B >= 1 && S >= 1 && KV >= 1 && H % KV == 0 && H >= KV && B * S < (1LL << 31) && B * H < (1LL << 24),
+              "sink attention: batch / heads");
+  TORCH_CHECK(window >= 1 && sinks >= 0, "sink attention: window >= 1, sinks >= 0");
+}
+
+std::vector<at::Tensor> sink_fwd(const at::Tensor& qkv, int64_t B, int64_t S, int64_t H, int64_t KV, int64_t D,
+                                 double scale, int64_t window, int64_t sinks, int64_t pad) {
+  need_sink_dims(B, S, H, KV, D, window, sinks);
+  need_packed(qkv, B, S, (H + 2 * KV) * D, "sink_fwd: qkv");
+  TORCH_CHECK(pad >= 0 && pad % 8 == 0, "sink_fwd: pad must be a multiple of 8");
+  c10::DeviceGuard guard(qkv.device());
+  auto obuf = at::empty({B * S, H * D + pad}, qkv.options());
+  auto o = pad ? obuf.narrow(1, 0, H * D) : obuf;
+  auto lse = at::empty({B, H, S}, qkv.options().dtype(at::kFloat));
+  const auto* p = static_cast<const uint16_t*>(qkv.data_ptr());
+  check(ftc_sink_fwd(p, p + H * D, p + (H + KV) * D, o.data_ptr(), lse.data_ptr<float>(), (int)B, (int)S, (int)H, (int)KV,
+                     (int)D, qkv.stride(0), qkv.stride(0), o.stride(0), (float)scale, (int)std::min(window, S),
+                     (int)std::min(sinks, S), cur_stream()),
+        "sink_fwd");
+  return {o, lse};
+}
+
+// gradient of the packed projection, [B*S, (H+2KV)*D] (the column view of a buffer with `pad` spare columns)
+at::Tensor sink_bwd(const at::Tensor& qkv, const at::Tensor& o, const at::Tensor& dout, const at::Tensor& lse, int64_t B,
+                    int64_t S, int64_t H, int64_t KV, int64_t D, double scale, int64_t window, int64_t sinks, int64_t pad,
+                    const c10::optional<at::Tensor>& rope_cos, const c10::optional<at::Tensor>& rope_sin,
+                    const c10::optional<at::Tensor>& rope_pos) {
+  need_sink_dims(B, S, H, KV, D, window, sinks);
+  const int64_t W = (H + 2 * KV) * D;
+  need_packed(qkv, B, S, W, "sink_bwd: qkv");
+  need_packed(o, B, S, H * D, "sink_bwd: o");
+  need_packed(dout, B, S, H * D, "sink_bwd: dout");
+  need(lse, at::kFloat, "sink_bwd: lse");
+  TORCH_CHECK(o.device() == qkv.device() && dout.device() == qkv.device() && lse.device() == qkv.device(),
+              "sink_bwd: tensors on one device");
+  TORCH_CHECK(lse.numel() == B * H * S && lse.is_contiguous(), "sink_bwd: lse [B, H, S]");
+  TORCH_CHECK(pad >= 0 && pad % 8 == 0, "sink_bwd: pad must be a multiple of 8");
+  const float *rc = nullptr, *rs = nullptr;
+  const int* rp = nullptr;
+  if (rope_cos.has_value()) {
+    TORCH_CHECK(rope_sin.has_value() && D == 128, "sink_bwd: rope_cos / rope_sin go together, head_dim 128");
+    for (auto* t : {&*rope_cos, &*rope_sin}) {
+      need(*t, at::kFloat, "sink_bwd: rope cos/sin");
+      TORCH_CHECK(t->dim() == 2 && t->size(1) == 64 && t->is_contiguous() && t->device() == qkv.device(),
+                  "sink_bwd: rope tables [max_pos, 64]");
+    }
+    rc = rope_cos->data_ptr<float>();
+    rs = rope_sin->data_ptr<float>();
+    if (rope_pos.has_value()) {
+      need(*rope_pos, at::kInt, "sink_bwd: rope_pos");
+      TORCH_CHECK(rope_pos->numel() == B * S && rope_pos->is_contiguous() && rope_pos->device() == qkv.device(),
+                  "sink_bwd: rope_pos [B*S]");
+      rp = rope_pos->data_ptr<int>();
+    } else {
+      TORCH_CHECK(rope_cos->size(0) >= S, "sink_bwd: rope tables shorter than the sequence");
+    }
+  }
+  c10::DeviceGuard guard(qkv.device());
+  auto buf = at::empty({B * S, W + pad}, qkv.options());
+  auto dqkv = pad ? buf.narrow(1, 0, W) : buf;
+  const int win = (int)std::min(window, S), snk = (int)std::min(sinks, S);
+  auto ws = at::empty({ftc_sink_bwd_workspace((int)B, (int)S, (int)H, (int)KV, (int)D, win, snk)},
+                      qkv.options().dtype(at::kFloat));
+  const auto* p = static_cast<const uint16_t*>(qkv.data_ptr());
+  auto* g = static_cast<uint16_t*>(dqkv.data_ptr());
+  check(ftc_sink_bwd(p, p + H * D, p + (H + KV) * D, o.data_ptr(), dout.data_ptr(), lse.data_ptr<float>(), g, g + H * D,
+                     g + (H + KV) * D, ws.data_ptr<float>(), (int)B, (int)S, (int)H, (int)KV, (int)D, qkv.stride(0),
+                     qkv.stride(0), o.stride(0), dout.stride(0), dqkv.stride(0), dqkv.stride(0), (float)scale, win, snk,
+                     rc, rs, rp, cur_stream()),
+        "sink_bwd");
+  return dqkv;
+}
+
 // ---------------- decode attention (generation) ----------------
 // qkv: [B, >=(H+2KV)*D] row view of the current token's packed projection (q | k | v); k_cache /
 // v_cache: [B, Lmax, KV*D] contiguous; lens: int32 [B] valid keys (current token included, <= max_len
@@ -874,6 +964,8 @@ PYBIND11_MODULE(_C, m) {
         py::arg("KV"), py::arg("D"), py::arg("scale"), py::arg("causal"), py::arg("window"),
         py::arg("doc_start") = py::none(), py::arg("doc_end") = py::none(), py::arg("kv_valid") = -1,
         py::arg("rope_cos") = py::none(), py::arg("rope_sin") = py::none(), py::arg("rope_pos") = py::none());
+  m.def("sink_fwd", &sink_fwd);
+  m.def("sink_bwd", &sink_bwd);
   m.def("decode_attention", &decode_attention);
   m.def("kv4_store_", &kv4_store_);
   m.def("kv4_load", &kv4_load);

@@ -21,7 +21,7 @@
 // tr_b16 column reads of V (guide T10 "one image for row reads and transposed reads").
 // Block order: heaviest causal q-blocks first; the G = H/KV query heads that share a kv head are
 // placed on the same XCD (blockIdx % 8 group) so their K/V tiles are L2 hits.
-#include "common.h"
+#include "flash_tiles.h"
 
 #include <cstdlib>
 #include <type_traits>
@@ -29,10 +29,6 @@
 using namespace ftc;
 
 namespace {
-
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 // query rows per workgroup = 32 x 4 waves (256 threads, two workgroups per CU).  Measured and removed
 // (git history, profiles/r1_attn_fwd_pp.log, profiles/r2/s9_attn_pipe*.log): 8 waves per workgroup
@@ -64,39 +60,6 @@ constexpr int BK = 64;   // keys per tile
 #define FWD_PK_SOFTMAX 0
 #endif
 typedef float f32x2 __attribute__((ext_vector_type(2)));
-constexpr float LOG2E = 1.4426950408889634f;
-constexpr float LN2 = 0.6931471805599453f;
-
-DEV_INLINE int swz(int r) { return ((r & 3) << 2) | ((r >> 2) & 3); }
-
-template <int D>
-DEV_INLINE int lds_off(int r, int chunk) {  // byte offset of 16-byte chunk `chunk` of row r
-  constexpr int NCH = D / 8;
-  return r * (D * 2) + 16 * ((chunk ^ swz(r)) & (NCH - 1));
-}
-
-DEV_INLINE bf16x8 as_bf8(const uint4& v) { return __builtin_bit_cast(bf16x8, v); }
-
-// max over lanes l and l ^ 32: v_permlane32_swap (gfx950 VALU, one instruction) instead of
-// ds_bpermute -- the row max sits on the softmax's dependency chain every tile, and the LDS permute's
-// round trip was part of it.
-DEV_INLINE float xhalf_max(float v) {
-  const auto pr = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  const float a = __uint_as_float(pr[0]), b = __uint_as_float(pr[1]);
-  return a > b ? a : b;  // lane l holds {v_l, v_(l^32)} in some order
-}
-
-DEV_INLINE bf16x8 pack_p(const f32x16& p, int base) {
-  f32x4 lo = {p[base + 0], p[base + 1], p[base + 2], p[base + 3]};
-  f32x4 hi = {p[base + 4], p[base + 5], p[base + 6], p[base + 7]};
-  uint4 u;
-  u.x = pack_bf2(lo[0], lo[1]);
-  u.y = pack_bf2(lo[2], lo[3]);
-  u.z = pack_bf2(hi[0], hi[1]);
-  u.w = pack_bf2(hi[2], hi[3]);
-  return as_bf8(u);
-}
-
 struct FwdArgs {
   const uint16_t* q;
   const uint16_t* k;
@@ -131,23 +94,6 @@ DEV_INLINE void decode_block(const FwdArgs& a, int& qb, int& b, int& hq, int& kv
   const int qr = t / a.B;
   qb = a.nqb - 1 - qr;  // heaviest (latest) query blocks first
   hq = kvh * G + g;
-}
-
-// One tile's K and V by LDS-DMA (buffer_load ... lds): NGT 1 KiB pieces per matrix per wave, the
-// lane's 16 bytes landing lane-linearly, the source pre-swizzled (voff) so the LDS image is the
-// XOR-swizzled one; toff = the tile's first row (scalar).  A device-only function: the host pass of
-// hipcc cannot instantiate these builtins inside a kernel lambda.
-template <int D, int NGT, int RPG>
-DEV_INLINE void fwd_dma(__amdgpu_buffer_rsrc_t kr, __amdgpu_buffer_rsrc_t vr, const int* voff, int toff, char* kdst,
-                     char* vdst, int wave) {
-#pragma unroll
-  for (int i = 0; i < NGT; ++i) {
-    const int r0 = (wave * NGT + i) * RPG;
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, (__attribute__((address_space(3))) void*)(kdst + r0 * D * 2), 16,
-                                             voff[i], toff, 0, 0);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, (__attribute__((address_space(3))) void*)(vdst + r0 * D * 2), 16,
-                                             voff[i], toff, 0, 0);
-  }
 }
 
 template <int D>
@@ -232,11 +178,11 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void flash_fwd_kernel(FwdArg
   if constexpr (FWD_EARLY_DMA) {
     // tile 0's K/V DMA first, then the Q loads: both latencies overlap (the first tile's vmcnt(0)
     // covers the two) instead of Q retiring before the DMA is issued
-    if (ntiles > 0) fwd_dma<D, NGT, RPG>(krs, vrs, voff, kv_begin * (int)a.kv_rs * 2, K0, V0, wave);
+    if (ntiles > 0) kv_dma<D, NGT, RPG>(krs, vrs, voff, kv_begin * (int)a.kv_rs * 2, K0, V0, wave);
     load_q();
   } else {
     __builtin_amdgcn_s_waitcnt(0x0F70);  // Q fragments (plain loads) retired before any DMA: vmcnt(0)
-    if (ntiles > 0) fwd_dma<D, NGT, RPG>(krs, vrs, voff, kv_begin * (int)a.kv_rs * 2, K0, V0, wave);
+    if (ntiles > 0) kv_dma<D, NGT, RPG>(krs, vrs, voff, kv_begin * (int)a.kv_rs * 2, K0, V0, wave);
   }
 
   // tr-read addressing (V^T A operand): 16-lane group gi = lane>>4 covers d cols [16*(gi&1), +16)
@@ -263,7 +209,7 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void flash_fwd_kernel(FwdArg
     __builtin_amdgcn_s_waitcnt(0x0F70);  // this wave's pieces of tile t landed (vmcnt(0))
     __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
     __builtin_amdgcn_s_barrier();        // ... and everyone's
-    if (t + 1 < ntiles) fwd_dma<D, NGT, RPG>(krs, vrs, voff, (kv_begin + (t + 1) * BK) * (int)a.kv_rs * 2, Kn, Vn, wave);
+    if (t + 1 < ntiles) kv_dma<D, NGT, RPG>(krs, vrs, voff, (kv_begin + (t + 1) * BK) * (int)a.kv_rs * 2, Kn, Vn, wave);
   };
   // ---- phase A: S^T = K Q^T, two 32-key blocks
   auto phaseA = [&](const char* Kc) __attribute__((always_inline)) {
@@ -364,7 +310,7 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void flash_fwd_kernel(FwdArg
     l += rs;
 #endif
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) pf[ks] = pack_p(s[ks >> 1], 8 * (ks & 1));
+    for (int ks = 0; ks < 4; ++ks) pf[ks] = pack8_bf(s[ks >> 1], 8 * (ks & 1));
   };
   // ---- phase B2: O^T += V^T P^T, 4 k-steps of 16 keys
   auto phaseB2 = [&](const char* Vc) __attribute__((always_inline)) {

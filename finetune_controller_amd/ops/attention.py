@@ -138,7 +138,7 @@ def _split(qkv, B, S, H, KV, D):
     return q, k, v
 
 
-def _sdpa_packed(qkv, B, S, H, KV, D, causal, window, scale, docs: Segments | None = None):
+def _sdpa_packed(qkv, B, S, H, KV, D, causal, window, scale, docs: Segments | None = None, sinks: int = 0):
     q, k, v = _split(qkv, B, S, H, KV, D)
     q = q.reshape(B, S, H, D).transpose(1, 2)
     k = k.reshape(B, S, KV, D).transpose(1, 2)
@@ -156,7 +156,7 @@ def _sdpa_packed(qkv, B, S, H, KV, D, causal, window, scale, docs: Segments | No
         o = F.scaled_dot_product_attention(q, k, v, attn_mask=mask, scale=scale)
     elif window and window > 0 and window < S:
         i = torch.arange(S, device=qkv.device)
-        allowed = (i[None, :] <= i[:, None]) & (i[:, None] - i[None, :] < window)
+        allowed = (i[None, :] <= i[:, None]) & ((i[:, None] - i[None, :] < window) | (i[None, :] < sinks))
         mask = allowed
         o = F.scaled_dot_product_attention(q, k, v, attn_mask=mask, scale=scale)
     else:
@@ -320,11 +320,70 @@ class _FlashPaddedTail(torch.autograd.Function):
         return dqkv, None, None, None, None, None, None, None, None, None, None, None
 
 
+class _FlashSinks(torch.autograd.Function):
+    """Window + sinks on ``csrc/kernels/flash_sink.hip``: any S; a head_dim the kernels are not built for runs on
+    zero-padded heads (exact: see _FlashPaddedTail)."""
+
+    @staticmethod
+    def forward(ctx, qkv, B, S, H, KV, D, window, sinks, scale, out_pad=0, grad_pad=0, rope_grad=None):
+        Dp = kernel_head_dim(D)
+        ctx.rope_grad = None
+        if Dp == D:
+            x = qkv
+            if x.stride(1) != 1 or x.stride(0) % 8 or x.data_ptr() % 16:
+                x = x.contiguous()
+                if x.data_ptr() % 16:
+                    x = x.clone()
+            o, lse = ext().sink_fwd(x, B, S, H, KV, D, scale, window, sinks, out_pad)
+            out = o
+            if rope_grad is not None and ROPE_BWD_FUSE and D == 128 and rope_grad.cos.shape[-1] == 64 and (
+                    rope_grad.pos is not None or rope_grad.cos.shape[0] >= S):
+                rope_grad.taken = True
+                ctx.rope_grad = rope_grad
+        else:
+            x = _pad_heads(qkv, B, S, S, H + 2 * KV, D, Dp)
+            o, lse = ext().sink_fwd(x, B, S, H, KV, Dp, scale, window, sinks, 0)
+            out = torch.empty(B * S, H * D + out_pad, dtype=qkv.dtype, device=qkv.device)[:, :H * D]
+            _unpad_heads(o, out, B, S, S, H, D, Dp)
+        ctx.save_for_backward(x, lse)
+        ctx.o = o.detach()  # outside save_for_backward, as in _FlashPacked (spare columns)
+        ctx.cfg = (B, S, H, KV, D, Dp, window, sinks, scale, grad_pad, qkv.shape[1])
+        return out
+
+    @staticmethod
+    def backward(ctx, do):
+        x, lse = ctx.saved_tensors
+        B, S, H, KV, D, Dp, window, sinks, scale, grad_pad, W = ctx.cfg
+        rg = ctx.rope_grad
+        nh = H + 2 * KV
+        _gate_dw()
+        if Dp == D:
+            if do.stride(1) != 1 or do.stride(0) % 8 or do.data_ptr() % 16:
+                do = do.contiguous()
+                if do.data_ptr() % 16:
+                    do = do.clone()
+            extra = W - nh * D  # qkv was wider than its heads: those columns get no gradient
+            g = ext().sink_bwd(x, ctx.o, do, lse, B, S, H, KV, D, scale, window, sinks, grad_pad if not extra else 0,
+                               rg.cos if rg is not None else None, rg.sin if rg is not None else None,
+                               rg.pos if rg is not None else None)
+            if extra:
+                g = torch.nn.functional.pad(g, (0, extra))
+        else:
+            gp = ext().sink_bwd(x, ctx.o, _pad_heads(do, B, S, S, H, D, Dp), lse, B, S, H, KV, Dp, scale, window, sinks, 0,
+                                None, None, None)
+            g = torch.zeros(B * S, W + grad_pad, dtype=x.dtype, device=x.device)[:, :W]
+            _unpad_heads(gp, g[:, :nh * D], B, S, S, nh, D, Dp)
+        return g, None, None, None, None, None, None, None, None, None, None, None
+
+
 def attention_packed(qkv: torch.Tensor, B: int, S: int, H: int, KV: int, D: int, causal: bool = True,
                      window: int = 0, scale: float | None = None, out_pad: int = 0,
                      grad_pad: int = 0, docs: Segments | None = None,
-                     rope_grad: RopeGrad | None = None) -> torch.Tensor:
+                     rope_grad: RopeGrad | None = None, sinks: int = 0) -> torch.Tensor:
     """Causal / sliding-window GQA attention on a packed ``[B*S, (H+2KV)*D]`` projection.
+
+    ``window`` > 0: query q sees the last ``window`` keys (itself included) and, with ``sinks`` > 0, the first
+    ``sinks`` keys of its sequence as well (causal only, one document per sequence).
 
     ``out_pad`` / ``grad_pad``: the output / the gradient of ``qkv`` are column views of
     row-padded buffers (spare columns for the augmented LoRA GEMMs, ``ops.linear``).  ``docs``: packed
@@ -332,18 +391,29 @@ def attention_packed(qkv: torch.Tensor, B: int, S: int, H: int, KV: int, D: int,
     scale = scale if scale is not None else 1.0 / math.sqrt(D)
     if docs is not None and not causal:
         raise ValueError("document-masked attention is causal")
-    if use_hip(qkv):
+    if sinks:
+        if sinks < 0:
+            raise ValueError(f"sinks must not be negative, got {sinks}")
+        if not causal or docs is not None:
+            raise ValueError("sinks: causal attention over one document per sequence only")
+        if not window or window <= 0:
+            sinks = 0  # every earlier key is seen anyway
+    if sinks and use_hip(qkv) and qkv.dtype == torch.bfloat16 and 0 < D <= 128 and B * S > 0:
+        return _FlashSinks.apply(qkv, B, S, H, KV, D, int(window), int(sinks), scale, out_pad, grad_pad, rope_grad)
+    if use_hip(qkv) and not sinks:
         if qkv.dtype == torch.bfloat16 and flash_supported(D, S):
             return _FlashPacked.apply(qkv, B, S, H, KV, D, causal, int(window or 0), scale, out_pad, grad_pad, docs,
                                       rope_grad)
         if qkv.dtype == torch.bfloat16 and flash_usable(D, S, causal):
             return _FlashPaddedTail.apply(qkv, B, S, H, KV, D, int(window or 0), scale, out_pad, grad_pad, docs,
                                           bool(causal))
+    if use_hip(qkv):
         _warn_fallback(f"dtype={qkv.dtype}, head_dim={D}, seq_len={S}, causal={causal}")
-    return _sdpa_packed(qkv, B, S, H, KV, D, causal, window, scale, docs)
+    return _sdpa_packed(qkv, B, S, H, KV, D, causal, window, scale, docs, sinks)
 
 
-def attention_reference(qkv, B, S, H, KV, D, causal=True, window=0, scale=None, docs: Segments | None = None):
+def attention_reference(qkv, B, S, H, KV, D, causal=True, window=0, scale=None, docs: Segments | None = None,
+                        sinks: int = 0):
     """fp32 math reference used by the kernel numerics tests."""
     scale = scale if scale is not None else 1.0 / math.sqrt(D)
     q, k, v = (t.float() for t in _split(qkv, B, S, H, KV, D))
@@ -356,7 +426,7 @@ def attention_reference(qkv, B, S, H, KV, D, causal=True, window=0, scale=None, 
     if causal:
         allowed &= i[None, :] <= i[:, None]
     if window and window > 0:
-        allowed &= (i[:, None] - i[None, :]) < window
+        allowed &= ((i[:, None] - i[None, :]) < window) | (i[None, :] < sinks)
     if docs is not None:
         allowed = allowed & _doc_mask(docs, B, S)
     s = s.masked_fill(~allowed, float("-inf"))

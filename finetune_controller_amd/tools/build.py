@@ -67,9 +67,11 @@ def _run(cmd: list[str]) -> None:
 #   of the softmax's f32 adds into v_pk_add_f32 (an anti-lever beside MFMAs: MI355X_MICROARCH.md cycle
 #   constants); the shipped 32-row kernel was measured with them in round 6, and the lab W64 build
 #   (tools/w64_lab/build.sh, which depends on them) uses the same
+#   flash_sink.hip -- as flash_attn_fwd.hip
 #   kv4_attn.hip -- MFMAs in VGPR form: with the accumulators in AGPRs the D = 128 kernel takes 166 registers (3
 #   waves per SIMD) instead of 128 (4)
 EXTRA_FLAGS = {"flash_attn_fwd.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-fno-slp-vectorize"],
+               "flash_sink.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-fno-slp-vectorize"],
                "kv4_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 
 

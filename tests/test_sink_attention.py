@@ -1,0 +1,229 @@
+"""Attention with a sliding window and sinks (ops.attention_packed(window=, sinks=)): query q sees key k iff k <= q and
+(q - k < window or k < sinks).  Forward and backward against the definition in 64 bits.
+
+Tolerances (bf16 tensors, half a step = 2^-8 relative; 32-bit sums and exponentials: 2^-12 of the summed magnitudes):
+  o    every p is rounded once, the output once:             2^-8 (sum p |v| + |o|)
+  dS   = p (dP - delta), delta from the rounded output:      p sum |do| tol_o, and the rounding of dS 2^-8 |dS|
+  dQ, dK  scale sum tol_dS |k|, |q|, the output's rounding 2^-8
+  dV   2^-8 (sum p |do| + |dV|)"""
+import math
+
+import pytest
+import torch
+
+from finetune_controller_amd import ops
+from finetune_controller_amd.ops.attention import RopeGrad
+
+BF, H8, SL = torch.bfloat16, 2.0 ** -8, 2.0 ** -12
+
+
+def _seen(S, window, sinks):
+    i = torch.arange(S)
+    d = i[:, None] - i[None, :]
+    return (d >= 0) & ((d < window) | (i[None, :] < sinks))
+
+
+def _definition(qkv, do, B, S, H, KV, D, window, sinks, scale):
+    """64-bit o and dqkv with their tolerances: (o, tol_o, g, tol_g), [B*S, ...]."""
+    x = qkv.detach().cpu().double()[:, :(H + 2 * KV) * D].view(B, S, H + 2 * KV, D)
+    dO = do.detach().cpu().double().view(B, S, H, D)
+    seen = _seen(S, window, sinks)
+    o, to = torch.zeros_like(dO), torch.zeros_like(dO)
+    g, tg = torch.zeros_like(x), torch.zeros_like(x)
+    for b in range(B):
+        for h in range(H):
+            kh, vh = H + h // (H // KV), H + KV + h // (H // KV)
+            q, k, v, d = x[b, :, h], x[b, :, kh], x[b, :, vh], dO[b, :, h]
+            p = torch.softmax((q @ k.T * scale).masked_fill(~seen, -math.inf), 1)
+            oh, pv = p @ v, p @ v.abs()
+            tol_o = H8 * (pv + oh.abs()) + SL * pv
+            dP = d @ v.T
+            delta = (d * oh).sum(1, keepdim=True)
+            dS = p * (dP - delta)
+            tS = p * ((d.abs() * tol_o).sum(1, keepdim=True) + SL * (d.abs() @ v.abs().T + delta.abs())) + H8 * dS.abs()
+            o[b, :, h], to[b, :, h] = oh, tol_o
+            g[b, :, h], tg[b, :, h] = scale * dS @ k, scale * tS @ k.abs()
+            g[b, :, kh] += scale * dS.T @ q
+            tg[b, :, kh] += scale * tS.T @ q.abs()
+            g[b, :, vh] += p.T @ d
+            tg[b, :, vh] += (H8 + SL) * p.T @ d.abs()
+    tg += H8 * g.abs()
+    return o.view(B * S, -1), to.view(B * S, -1), g.view(B * S, -1), tg.view(B * S, -1)
+
+
+def _inputs(B, S, H, KV, D, seed=0, dtype=BF):
+    g = torch.Generator().manual_seed(seed)
+    qkv = torch.randn(B * S, (H + 2 * KV) * D, generator=g)
+    qkv[:, :(H + KV) * D] *= 1.3
+    return qkv.to(dtype), torch.randn(B * S, H * D, generator=g).to(dtype)
+
+
+def _close(got, want, tol):
+    err = (got.detach().double().cpu() - want).abs()
+    assert err.isfinite().all()
+    assert (err <= tol).all(), float((err / tol.clamp_min(1e-30)).max())
+
+
+# ---------------------------------------------------------------- torch path
+@pytest.mark.parametrize("S,window,sinks", [(1, 1, 1), (9, 3, 2), (20, 1, 4), (20, 7, 30), (17, 40, 3), (16, 5, 0)])
+def test_torch_path_matches_the_definition(S, window, sinks):
+    B, H, KV, D = 2, 4, 2, 8
+    qkv, do = _inputs(B, S, H, KV, D, dtype=torch.float64)
+    qkv.requires_grad_()
+    o = ops.attention_packed(qkv, B, S, H, KV, D, window=window, sinks=sinks)
+    (g,) = torch.autograd.grad(o, qkv, do)
+    wo, _, wg, _ = _definition(qkv, do, B, S, H, KV, D, window, sinks, D ** -0.5)
+    torch.testing.assert_close(o.detach(), wo, atol=1e-12, rtol=1e-12)
+    torch.testing.assert_close(g, wg, atol=1e-12, rtol=1e-12)
+    torch.testing.assert_close(ops.attention_reference(qkv.detach(), B, S, H, KV, D, window=window, sinks=sinks).double(), wo,
+                               atol=1e-5, rtol=1e-5)
+
+
+def test_gradient_against_differences():
+    B, S, H, KV, D = 1, 7, 2, 1, 4
+    qkv, _ = _inputs(B, S, H, KV, D, dtype=torch.float64)
+    assert torch.autograd.gradcheck(lambda x: ops.attention_packed(x, B, S, H, KV, D, window=2, sinks=1), qkv.requires_grad_())
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_refusals(dev):
+    qkv = torch.zeros(8, 4 * 64, dtype=BF, device=dev)
+    with pytest.raises(ValueError, match="negative"):
+        ops.attention_packed(qkv, 1, 8, 2, 1, 64, window=4, sinks=-1)
+    with pytest.raises(ValueError, match="causal"):
+        ops.attention_packed(qkv, 1, 8, 2, 1, 64, False, window=4, sinks=1)
+    docs = ops.segments_from_eos(torch.zeros(1, 8, dtype=torch.long, device=dev), 5)
+    with pytest.raises(ValueError, match="one document"):
+        ops.attention_packed(qkv, 1, 8, 2, 1, 64, window=4, sinks=1, docs=docs)
+
+
+# ---------------------------------------------------------------- kernels
+SHAPES = [  # B, S, H, KV, D, window, sinks
+    (1, 1, 1, 1, 128, 1, 1),
+    (2, 33, 2, 1, 64, 5, 1),
+    (1, 64, 2, 2, 128, 64, 7),
+    (1, 129, 4, 1, 64, 1, 64),
+    (2, 257, 2, 1, 128, 17, 4),
+    (1, 300, 3, 3, 64, 100, 65),
+    (1, 511, 4, 2, 128, 128, 3),
+    (3, 640, 2, 1, 64, 33, 33),
+    (1, 1025, 2, 1, 128, 300, 300),
+    (1, 1300, 2, 2, 128, 40, 260),
+    (1, 600, 6, 3, 80, 50, 5),
+    (2, 77, 2, 1, 32, 9, 2),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,S,H,KV,D,window,sinks", SHAPES)
+def test_kernels(B, S, H, KV, D, window, sinks):
+    qkv, do = _inputs(B, S, H, KV, D, seed=S)
+    x = qkv.cuda().requires_grad_()
+    scale = 0.7 / math.sqrt(D)
+    o = ops.attention_packed(x, B, S, H, KV, D, window=window, sinks=sinks, scale=scale)
+    (g,) = torch.autograd.grad(o, x, do.cuda())
+    wo, to, wg, tg = _definition(qkv, do, B, S, H, KV, D, window, sinks, scale)
+    assert o.dtype == BF and g.dtype == BF and o.shape == (B * S, H * D) and g.shape == qkv.shape
+    _close(o, wo, to)
+    _close(g, wg, tg)
+    # against differences of the 64-bit function, along one direction
+    d = torch.randn(qkv.shape, generator=torch.Generator().manual_seed(1)).double()
+    e, xd = 1e-6, qkv.double()
+    up, dn = (_definition(xd + t * e * d, do, B, S, H, KV, D, window, sinks, scale)[0] for t in (1, -1))
+    diff = float(((up - dn) * do.double()).sum() / (2 * e))
+    assert abs(float((g.double().cpu() * d).sum()) - diff) <= float((tg * d.abs()).sum()) + 1e-5 * abs(diff) + 1e-4
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("S,window", [(512, 100), (300, 512)])
+def test_views_and_padded_buffers(S, window):
+    """A row-padded projection, padded output and gradient buffers, an output gradient with odd strides."""
+    B, H, KV, D, sinks = 1, 4, 2, 128, 4
+    W = (H + 2 * KV) * D
+    qkv, do = _inputs(B, S, H, KV, D, seed=3)
+    wo, to, wg, tg = _definition(qkv, do, B, S, H, KV, D, window, sinks, D ** -0.5)
+    buf = torch.full((B * S, W + 24), math.nan, dtype=BF, device="cuda")
+    buf[:, :W] = qkv.cuda()
+    leaf = buf.requires_grad_()
+    o = ops.attention_packed(leaf[:, :W], B, S, H, KV, D, window=window, sinks=sinks, out_pad=64, grad_pad=64)
+    assert o.stride(0) == H * D + 64
+    odd = torch.empty(B * S, H * D + 3, dtype=BF, device="cuda")[:, 1:H * D + 1]
+    odd.copy_(do.cuda())
+    (g,) = torch.autograd.grad(o, leaf, odd)
+    _close(o, wo, to)
+    _close(g[:, :W], wg, tg)
+    x = torch.empty(B * S * W + 1, dtype=BF, device="cuda")[1:].view(B * S, W).copy_(qkv.cuda()).requires_grad_()  # off 16 bytes
+    (g2,) = torch.autograd.grad(ops.attention_packed(x, B, S, H, KV, D, window=window, sinks=sinks), x, do.cuda())
+    assert torch.equal(g2, g[:, :W])
+    wide = leaf.detach().requires_grad_()  # more columns than heads: their gradient is zero
+    (g3,) = torch.autograd.grad(ops.attention_packed(wide, B, S, H, KV, D, window=window, sinks=sinks), wide, do.cuda())
+    assert torch.equal(g3[:, :W], g2) and (g3[:, W:] == 0).all()
+
+
+@pytest.mark.gpu
+def test_rope_handoff():
+    """The backward takes RoPE's inverse rotation into its epilogues (rows past a tile, positions given)."""
+    B, S, H, KV, D, window, sinks = 2, 290, 2, 1, 128, 64, 4
+    qkv, do = _inputs(B, S, H, KV, D, seed=9)
+    table = ops.RotaryTable(D, 512)
+    cos, sin = table.get("cuda")
+    pos = (torch.arange(S) + 11).repeat(B).to(torch.int32).cuda()
+    for p in (None, pos):
+        rg = RopeGrad(cos, sin, p)
+        x = qkv.cuda().requires_grad_()
+        o = ops.attention_packed(x, B, S, H, KV, D, window=window, sinks=sinks, rope_grad=rg)
+        assert rg.taken
+        (g,) = torch.autograd.grad(o, x, do.cuda())
+        _, _, wg, tg = _definition(qkv, do, B, S, H, KV, D, window, sinks, D ** -0.5)
+        idx = (torch.arange(S).repeat(B) if p is None else p.cpu()).long()
+        c, s = cos.cpu().double()[idx][:, None], sin.cpu().double()[idx][:, None]
+        n = H + KV
+        a, t = (z[:, :n * D].reshape(B * S, n, D) for z in (wg, tg))
+        rot = torch.cat([a[..., :64] * c + a[..., 64:] * s, a[..., 64:] * c - a[..., :64] * s], -1)
+        tr = t[..., :64] + t[..., 64:]
+        _close(g[:, :n * D], rot.reshape(B * S, -1), torch.cat([tr, tr], -1).reshape(B * S, -1))
+        _close(g[:, n * D:], wg[:, n * D:], tg[:, n * D:])
+
+
+@pytest.mark.gpu
+def test_reproducible_on_a_side_stream_and_in_a_graph():
+    B, S, H, KV, D, window, sinks = 1, 700, 4, 1, 128, 90, 5
+    qkv, do = (t.cuda() for t in _inputs(B, S, H, KV, D, seed=4))
+
+    def step(x, d):
+        x = x.detach().requires_grad_()
+        o = ops.attention_packed(x, B, S, H, KV, D, window=window, sinks=sinks)
+        return o.detach(), torch.autograd.grad(o, x, d)[0]
+
+    want = [step(qkv * s, do) for s in (1.0, 0.5, 2.0)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step(qkv, do)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(got, want[0]))
+    xin = qkv.clone()
+    with torch.cuda.stream(side):
+        step(xin, do)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(xin, do)
+    for s, w in zip((1.0, 0.5, 2.0), want):
+        xin.copy_(qkv * s)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, w)), s
+
+
+@pytest.mark.gpu
+def test_everything_in_the_window_equals_causal_attention():
+    B, S, H, KV, D = 1, 512, 4, 2, 128
+    qkv, do = (t.cuda() for t in _inputs(B, S, H, KV, D, seed=6))
+    wo, to, wg, tg = _definition(qkv, do, B, S, H, KV, D, S, 0, D ** -0.5)
+    for window, sinks in ((S, 4), (3, S), (10 ** 9, 10 ** 9)):
+        x = qkv.detach().requires_grad_()
+        o = ops.attention_packed(x, B, S, H, KV, D, window=window, sinks=sinks)
+        (g,) = torch.autograd.grad(o, x, do)
+        _close(o, wo, to)
+        _close(g, wg, tg)
