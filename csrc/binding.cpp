@@ -61,10 +61,10 @@ int ftc_flash_bwd(const void* q, const void* k, const void* v, const void* o, co
                   long long dkv_row_stride, float scale, int causal, int window, const int* doc_start,
                   const int* doc_end, int kv_valid, const float* rope_cos, const float* rope_sin,
                   const int* rope_pos, hipStream_t stream);
-int ftc_sink_fwd(const void* q, const void* k, const void* v, void* o, float* lse, int B, int S, int H, int KV, int D,
+int ftc_sink_fwd(const void* q, const void* k, const void* v, void* o, void* olow, float* lse, int B, int S, int H, int KV, int D,
                  long long q_rs, long long kv_rs, long long o_rs, float scale, int window, int sinks, hipStream_t stream);
 long long ftc_sink_bwd_workspace(int B, int S, int H, int KV, int D, int window, int sinks);
-int ftc_sink_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, const float* lse, void* dq,
+int ftc_sink_bwd(const void* q, const void* k, const void* v, const void* o, const void* olow, const void* dout, const float* lse, void* dq,
                  void* dk, void* dv, float* workspace, int B, int S, int H, int KV, int D, long long q_rs, long long kv_rs,
                  long long o_rs, long long do_rs, long long dq_rs, long long dkv_rs, float scale, int window, int sinks,
                  const float* rope_cos, const float* rope_sin, const int* rope_pos, hipStream_t stream);
@@ -546,6 +546,7 @@ void flash_bwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, co
 
 // ---------------- flash attention with a window and sinks (csrc/kernels/flash_sink.hip) ----------------
 // q, k, v are head-column views of one packed [B*S, (H+2KV)*D] projection (16-byte aligned rows), any S.
+// grad: the output's low bits (uint8, a [0, H*D] tensor otherwise) are kept for the backward.
 inline void need_packed(const at::Tensor& qkv, int64_t B, int64_t S, int64_t W, const char* name) {
   need(qkv, at::kBFloat16, name);
   TORCH_CHECK(qkv.dim() == 2 && qkv.size(0) == B * S && qkv.size(1) >= W && qkv.stride(1) == 1 &&
@@ -560,7 +561,7 @@ inline void need_sink_dims(int64_t B, int64_t S, int64_t H, int64_t KV, int64_t 
 }
 
 std::vector<at::Tensor> sink_fwd(const at::Tensor& qkv, int64_t B, int64_t S, int64_t H, int64_t KV, int64_t D,
-                                 double scale, int64_t window, int64_t sinks, int64_t pad) {
+                                 double scale, int64_t window, int64_t sinks, int64_t pad, bool grad) {
   need_sink_dims(B, S, H, KV, D, window, sinks);
   need_packed(qkv, B, S, (H + 2 * KV) * D, "sink_fwd: qkv");
   TORCH_CHECK(pad >= 0 && pad % 8 == 0, "sink_fwd: pad must be a multiple of 8");
@@ -568,17 +569,18 @@ std::vector<at::Tensor> sink_fwd(const at::Tensor& qkv, int64_t B, int64_t S, in
   auto obuf = at::empty({B * S, H * D + pad}, qkv.options());
   auto o = pad ? obuf.narrow(1, 0, H * D) : obuf;
   auto lse = at::empty({B, H, S}, qkv.options().dtype(at::kFloat));
+  auto olow = at::empty({grad ? B * S : 0, H * D}, qkv.options().dtype(at::kByte));
   const auto* p = static_cast<const uint16_t*>(qkv.data_ptr());
-  check(ftc_sink_fwd(p, p + H * D, p + (H + KV) * D, o.data_ptr(), lse.data_ptr<float>(), (int)B, (int)S, (int)H, (int)KV,
+  check(ftc_sink_fwd(p, p + H * D, p + (H + KV) * D, o.data_ptr(), grad ? olow.data_ptr() : nullptr, lse.data_ptr<float>(), (int)B, (int)S, (int)H, (int)KV,
                      (int)D, qkv.stride(0), qkv.stride(0), o.stride(0), (float)scale, (int)std::min(window, S),
                      (int)std::min(sinks, S), cur_stream()),
         "sink_fwd");
-  return {o, lse};
+  return {o, olow, lse};
 }
 
 // gradient of the packed projection, [B*S, (H+2KV)*D] (the column view of a buffer with `pad` spare columns)
-at::Tensor sink_bwd(const at::Tensor& qkv, const at::Tensor& o, const at::Tensor& dout, const at::Tensor& lse, int64_t B,
-                    int64_t S, int64_t H, int64_t KV, int64_t D, double scale, int64_t window, int64_t sinks, int64_t pad,
+at::Tensor sink_bwd(const at::Tensor& qkv, const at::Tensor& o, const at::Tensor& olow, const at::Tensor& dout,
+                    const at::Tensor& lse, int64_t B, int64_t S, int64_t H, int64_t KV, int64_t D, double scale, int64_t window, int64_t sinks, int64_t pad,
                     const c10::optional<at::Tensor>& rope_cos, const c10::optional<at::Tensor>& rope_sin,
                     const c10::optional<at::Tensor>& rope_pos) {
   need_sink_dims(B, S, H, KV, D, window, sinks);
@@ -587,6 +589,10 @@ at::Tensor sink_bwd(const at::Tensor& qkv, const at::Tensor& o, const at::Tensor
   need_packed(o, B, S, H * D, "sink_bwd: o");
   need_packed(dout, B, S, H * D, "sink_bwd: dout");
   need(lse, at::kFloat, "sink_bwd: lse");
+  need(olow, at::kByte, "sink_bwd: olow");
+  TORCH_CHECK(olow.dim() == 2 && olow.size(0) == B * S && olow.size(1) == H * D && olow.is_contiguous() &&
+                  olow.device() == qkv.device() && reinterpret_cast<uintptr_t>(olow.data_ptr()) % 16 == 0,
+              "sink_bwd: olow [B*S, H*D]");
   TORCH_CHECK(o.device() == qkv.device() && dout.device() == qkv.device() && lse.device() == qkv.device(),
               "sink_bwd: tensors on one device");
   TORCH_CHECK(lse.numel() == B * H * S && lse.is_contiguous(), "sink_bwd: lse [B, H, S]");
@@ -619,8 +625,8 @@ at::Tensor sink_bwd(const at::Tensor& qkv, const at::Tensor& o, const at::Tensor
                       qkv.options().dtype(at::kFloat));
   const auto* p = static_cast<const uint16_t*>(qkv.data_ptr());
   auto* g = static_cast<uint16_t*>(dqkv.data_ptr());
-  check(ftc_sink_bwd(p, p + H * D, p + (H + KV) * D, o.data_ptr(), dout.data_ptr(), lse.data_ptr<float>(), g, g + H * D,
-                     g + (H + KV) * D, ws.data_ptr<float>(), (int)B, (int)S, (int)H, (int)KV, (int)D, qkv.stride(0),
+  check(ftc_sink_bwd(p, p + H * D, p + (H + KV) * D, o.data_ptr(), olow.data_ptr(), dout.data_ptr(), lse.data_ptr<float>(), g,
+                     g + H * D, g + (H + KV) * D, ws.data_ptr<float>(), (int)B, (int)S, (int)H, (int)KV, (int)D, qkv.stride(0),
                      qkv.stride(0), o.stride(0), dout.stride(0), dqkv.stride(0), dqkv.stride(0), (float)scale, win, snk,
                      rc, rs, rp, cur_stream()),
         "sink_bwd");

@@ -25,6 +25,7 @@ struct FwdArgs {
   const uint16_t* k;
   const uint16_t* v;
   uint16_t* o;
+  uint8_t* olow;  // [B*S, H*D] GRAD: the 8 significand bits of O below bf16's (low_byte)
   float* lse;
   long long q_rs, kv_rs, o_rs;
   int B, S, H, KV, nqb;
@@ -54,7 +55,22 @@ DEV_INLINE void decode_block(const FwdArgs& a, int& qb, int& b, int& hq, int& kv
   hq = kvh * G + g;
 }
 
-template <int D>
+// Signed distance of a float from its bf16 rounding in units of 2^-8 of a bf16 step, as a byte, and back: with it O
+// has a 16-bit significand.  The backward's delta = rowsum(dO * O) cancels against dP; from the rounded O alone it put
+// half again the other roundings' error into dQ and dK (relative error of dqkv 0.0028 against 64 bits, 0.0024 with the
+// byte; the output's own rounding is 0.0017).
+DEV_INLINE uint32_t low_byte(float x) {
+  const int r = (int)(__float_as_uint(x) - ((uint32_t)f2bf(x) << 16)) >> 8;
+  return (uint32_t)min(r, 127) & 0xffu;
+}
+DEV_INLINE float with_low_byte(uint32_t hi, uint32_t byte) {  // hi: the bf16 in the high half
+  return __uint_as_float(hi + ((uint32_t)((int)(byte << 24) >> 24) << 8));
+}
+
+// GRAD: the output is for a backward pass as well: its low bits are kept, and O is normalised by the sum of the weights
+// as they were rounded for the PV product (one more MFMA column of ones), so that the rounding of a row's largest
+// weights cancels; the LSE keeps the 32-bit sum.
+template <int D, bool GRAD>
 __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void sink_fwd_kernel(FwdArgs a) {
   constexpr int BQ = 32 * WAVES;
   constexpr int NCH = D / 8;           // 16-byte chunks per row
@@ -131,6 +147,8 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void sink_fwd_kernel(FwdArgs
     for (int i = 0; i < 16; ++i) o[t][i] = 0.f;
   float m = -INFINITY, l = 0.f;
   const float c = a.scale_log2;
+  f32x16 lr_ = {};  // GRAD: sum of the rounded weights (every element)
+  const bf16x8 ones = as_bf8(make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u));
 
   __builtin_amdgcn_s_waitcnt(0x0F70);  // Q fragments (plain loads) retired before any DMA: vmcnt(0)
   dma(tile_key(0), K0, V0);
@@ -223,6 +241,10 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void sink_fwd_kernel(FwdArgs
       for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[dt][i] *= alpha;
+      if constexpr (GRAD) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) lr_[i] *= alpha;
+      }
     }
     const float mref = (m == -INFINITY) ? 0.f : m;
     float rs = 0.f;
@@ -240,6 +262,10 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void sink_fwd_kernel(FwdArgs
   };
   // ---- phase B2: O^T += V^T P^T, 4 k-steps of 16 keys
   auto phaseB2 = [&](const char* Vc) __attribute__((always_inline)) {
+    if constexpr (GRAD) {
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) lr_ = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ones, pf[ks], lr_, 0, 0, 0);
+    }
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
       s16x4 vt[8];  // all 8 transposed reads of this 32-wide d tile in flight before the MFMA chain
@@ -273,8 +299,23 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void sink_fwd_kernel(FwdArgs
 
   // ---- epilogue: normalise, store O (bf16) and LSE (natural log)
   const float ltot = l + __shfl_xor(l, 32, 64);
-  const float inv = ltot > 0.f ? 1.0f / ltot : 0.f;
+  const float lnorm = GRAD ? lr_[0] : ltot, inv = lnorm > 0.f ? 1.0f / lnorm : 0.f;
   uint16_t* op = a.o + ((long long)b * S + (qvalid ? qrow : 0)) * a.o_rs + (long long)hq * D;
+  if constexpr (GRAD) {
+    // the 4 bytes of each g4 are a dword; two swaps give lane half hh the 16 bytes of d [16 hh, 16 hh + 16)
+    uint8_t* lp = a.olow + ((long long)b * S + (qvalid ? qrow : 0)) * ((long long)a.H * D) + (long long)hq * D;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      uint32_t w[4];
+#pragma unroll
+      for (int g4 = 0; g4 < 4; ++g4)
+        w[g4] = low_byte(o[dt][4 * g4] * inv) | low_byte(o[dt][4 * g4 + 1] * inv) << 8 |
+                low_byte(o[dt][4 * g4 + 2] * inv) << 16 | low_byte(o[dt][4 * g4 + 3] * inv) << 24;
+      const auto a0 = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
+      const auto b0 = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
+      if (qvalid) *reinterpret_cast<uint4*>(lp + dt * 32 + 16 * hh) = make_uint4(a0[0], a0[1], b0[0], b0[1]);
+    }
+  }
   if ((a.o_rs & 7) == 0) {
     // 16-byte stores (the store tail is issue-bound): lanes l and l ^ 32 hold the same
     // query row, d runs {8 g4 + 4 hh + 0..3}; two v_permlane32_swap per dword pair give lane half hh
@@ -322,6 +363,7 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void sink_fwd_kernel(FwdArgs
 // ---------------------------------------------------------------- backward
 struct BwdArgs {
   const uint16_t *q, *k, *v, *o, *dout;
+  const uint8_t* olow;  // O's bits below bf16's (low_byte)
   const float* lse;
   float* delta;  // workspace [-delta | -lse/scale], B*H*S each
   uint16_t *dq, *dk, *dv;
@@ -813,13 +855,17 @@ __global__ __launch_bounds__(256, 2) void sink_dq_kernel(BwdArgs a) {
   float dsum = 0.f;
   {
     const uint16_t* op = a.o + ((long long)b * S + qrow) * a.o_rs + (long long)hq * D + 8 * hh;
+    const uint8_t* lp = a.olow + ((long long)b * S + qrow) * ((long long)a.H * D) + (long long)hq * D + 8 * hh;
 #pragma unroll
     for (int s = 0; s < DSTEPS; ++s) {
-      float fo[8], fd[8];
-      unpack8(*reinterpret_cast<const uint4*>(op + 16 * s), fo);
+      float fd[8];
+      const uint4 u = *reinterpret_cast<const uint4*>(op + 16 * s);
+      const uint2 w = *reinterpret_cast<const uint2*>(lp + 16 * s);
+      const uint32_t hi[4] = {u.x, u.y, u.z, u.w}, lo[2] = {w.x, w.y};
       unpack8(__builtin_bit_cast(uint4, df[s]), fd);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) dsum += fo[j] * fd[j];
+      for (int j = 0; j < 8; ++j)
+        dsum += with_low_byte(j & 1 ? hi[j >> 1] & 0xffff0000u : hi[j >> 1] << 16, (lo[j >> 2] >> (8 * (j & 3))) & 0xffu) * fd[j];
     }
   }
   dsum += __shfl_xor(dsum, 32, 64);
@@ -945,7 +991,7 @@ __global__ __launch_bounds__(256, 2) void sink_dq_kernel(BwdArgs a) {
 
 }  // namespace
 
-extern "C" int ftc_sink_fwd(const void* q, const void* k, const void* v, void* o, float* lse, int B, int S, int H, int KV,
+extern "C" int ftc_sink_fwd(const void* q, const void* k, const void* v, void* o, void* olow, float* lse, int B, int S, int H, int KV,
                             int D, long long q_rs, long long kv_rs, long long o_rs, float scale, int window, int sinks,
                             hipStream_t stream) {
   // the rows of one (batch, kv head) are addressed with 32-bit buffer offsets
@@ -953,14 +999,17 @@ extern "C" int ftc_sink_fwd(const void* q, const void* k, const void* v, void* o
       (long long)S * kv_rs * 2 >= (1LL << 31))
     return -1;
   const int BQ = 32 * WAVES;
-  FwdArgs a{(const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, (uint16_t*)o, lse, q_rs, kv_rs, o_rs,
-            B, S, H, KV, (S + BQ - 1) / BQ, scale * LOG2E, window < S ? window : S, sinks < S ? sinks : S};
+  FwdArgs a{(const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, (uint16_t*)o, (uint8_t*)olow, lse, q_rs,
+            kv_rs, o_rs, B, S, H, KV, (S + BQ - 1) / BQ, scale * LOG2E, window < S ? window : S, sinks < S ? sinks : S};
   const long long blocks = (long long)a.nqb * B * H;
   if (blocks > 0x7fffffffLL) return -1;
-  if (D == 128)
-    hipLaunchKernelGGL((sink_fwd_kernel<128>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
-  else
-    hipLaunchKernelGGL((sink_fwd_kernel<64>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
+  if (D == 128) {
+    if (olow) hipLaunchKernelGGL((sink_fwd_kernel<128, true>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((sink_fwd_kernel<128, false>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
+  } else {
+    if (olow) hipLaunchKernelGGL((sink_fwd_kernel<64, true>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((sink_fwd_kernel<64, false>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
+  }
   return (int)hipGetLastError();
 }
 
@@ -981,8 +1030,8 @@ extern "C" long long ftc_sink_bwd_workspace(int B, int S, int H, int KV, int D, 
   return base + (long long)B * KV * far_parts(B, S, H, KV, window, sinks) * n * 2 * D;
 }
 
-extern "C" int ftc_sink_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, const float* lse,
-                            void* dq, void* dk, void* dv, float* workspace, int B, int S, int H, int KV, int D,
+extern "C" int ftc_sink_bwd(const void* q, const void* k, const void* v, const void* o, const void* olow, const void* dout,
+                            const float* lse, void* dq, void* dk, void* dv, float* workspace, int B, int S, int H, int KV, int D,
                             long long q_rs, long long kv_rs, long long o_rs, long long do_rs, long long dq_rs,
                             long long dkv_rs, float scale, int window, int sinks, const float* rope_cos,
                             const float* rope_sin, const int* rope_pos, hipStream_t stream) {
@@ -995,7 +1044,7 @@ extern "C" int ftc_sink_bwd(const void* q, const void* k, const void* v, const v
   if ((long long)S * max_rs * 2 >= (1LL << 31) || 2LL * B * H * S * 4 >= (1LL << 31)) return -1;
   const int nfar = far_parts(B, S, H, KV, window, sinks);
   BwdArgs a{(const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, (const uint16_t*)o, (const uint16_t*)dout,
-            lse, workspace, (uint16_t*)dq, (uint16_t*)dk, (uint16_t*)dv, q_rs, kv_rs, o_rs, dq_rs, dkv_rs, do_rs,
+            (const uint8_t*)olow, lse, workspace, (uint16_t*)dq, (uint16_t*)dk, (uint16_t*)dv, q_rs, kv_rs, o_rs, dq_rs, dkv_rs, do_rs,
             B, S, H, KV, scale, scale * LOG2E, window < S ? window : S, sinks < S ? sinks : S,
             nfar ? workspace + (2LL * B * H * S + 3) / 4 * 4 : nullptr, nfar, rope_cos, rope_sin, rope_pos};
   const dim3 g_kv(B * KV * ((S + 255) / 256)), g_q(B * H * ((S + 127) / 128));

@@ -325,7 +325,8 @@ class _FlashSinks(torch.autograd.Function):
     zero-padded heads (exact: see _FlashPaddedTail)."""
 
     @staticmethod
-    def forward(ctx, qkv, B, S, H, KV, D, window, sinks, scale, out_pad=0, grad_pad=0, rope_grad=None):
+    def forward(ctx, qkv, B, S, H, KV, D, window, sinks, scale, out_pad=0, grad_pad=0, rope_grad=None, grad=True):
+        grad = grad and ctx.needs_input_grad[0]
         Dp = kernel_head_dim(D)
         ctx.rope_grad = None
         if Dp == D:
@@ -334,7 +335,7 @@ class _FlashSinks(torch.autograd.Function):
                 x = x.contiguous()
                 if x.data_ptr() % 16:
                     x = x.clone()
-            o, lse = ext().sink_fwd(x, B, S, H, KV, D, scale, window, sinks, out_pad)
+            o, olow, lse = ext().sink_fwd(x, B, S, H, KV, D, scale, window, sinks, out_pad, grad)
             out = o
             if rope_grad is not None and ROPE_BWD_FUSE and D == 128 and rope_grad.cos.shape[-1] == 64 and (
                     rope_grad.pos is not None or rope_grad.cos.shape[0] >= S):
@@ -342,17 +343,17 @@ class _FlashSinks(torch.autograd.Function):
                 ctx.rope_grad = rope_grad
         else:
             x = _pad_heads(qkv, B, S, S, H + 2 * KV, D, Dp)
-            o, lse = ext().sink_fwd(x, B, S, H, KV, Dp, scale, window, sinks, 0)
+            o, olow, lse = ext().sink_fwd(x, B, S, H, KV, Dp, scale, window, sinks, 0, grad)
             out = torch.empty(B * S, H * D + out_pad, dtype=qkv.dtype, device=qkv.device)[:, :H * D]
             _unpad_heads(o, out, B, S, S, H, D, Dp)
-        ctx.save_for_backward(x, lse)
+        ctx.save_for_backward(x, olow, lse)
         ctx.o = o.detach()  # outside save_for_backward, as in _FlashPacked (spare columns)
         ctx.cfg = (B, S, H, KV, D, Dp, window, sinks, scale, grad_pad, qkv.shape[1])
         return out
 
     @staticmethod
     def backward(ctx, do):
-        x, lse = ctx.saved_tensors
+        x, olow, lse = ctx.saved_tensors
         B, S, H, KV, D, Dp, window, sinks, scale, grad_pad, W = ctx.cfg
         rg = ctx.rope_grad
         nh = H + 2 * KV
@@ -363,17 +364,17 @@ class _FlashSinks(torch.autograd.Function):
                 if do.data_ptr() % 16:
                     do = do.clone()
             extra = W - nh * D  # qkv was wider than its heads: those columns get no gradient
-            g = ext().sink_bwd(x, ctx.o, do, lse, B, S, H, KV, D, scale, window, sinks, grad_pad if not extra else 0,
+            g = ext().sink_bwd(x, ctx.o, olow, do, lse, B, S, H, KV, D, scale, window, sinks, grad_pad if not extra else 0,
                                rg.cos if rg is not None else None, rg.sin if rg is not None else None,
                                rg.pos if rg is not None else None)
             if extra:
                 g = torch.nn.functional.pad(g, (0, extra))
         else:
-            gp = ext().sink_bwd(x, ctx.o, _pad_heads(do, B, S, S, H, D, Dp), lse, B, S, H, KV, Dp, scale, window, sinks, 0,
-                                None, None, None)
+            gp = ext().sink_bwd(x, ctx.o, olow, _pad_heads(do, B, S, S, H, D, Dp), lse, B, S, H, KV, Dp, scale, window,
+                                sinks, 0, None, None, None)
             g = torch.zeros(B * S, W + grad_pad, dtype=x.dtype, device=x.device)[:, :W]
             _unpad_heads(gp, g[:, :nh * D], B, S, S, nh, D, Dp)
-        return g, None, None, None, None, None, None, None, None, None, None, None
+        return g, None, None, None, None, None, None, None, None, None, None, None, None
 
 
 def attention_packed(qkv: torch.Tensor, B: int, S: int, H: int, KV: int, D: int, causal: bool = True,
@@ -399,7 +400,8 @@ def attention_packed(qkv: torch.Tensor, B: int, S: int, H: int, KV: int, D: int,
         if not window or window <= 0:
             sinks = 0  # every earlier key is seen anyway
     if sinks and use_hip(qkv) and qkv.dtype == torch.bfloat16 and 0 < D <= 128 and B * S > 0:
-        return _FlashSinks.apply(qkv, B, S, H, KV, D, int(window), int(sinks), scale, out_pad, grad_pad, rope_grad)
+        return _FlashSinks.apply(qkv, B, S, H, KV, D, int(window), int(sinks), scale, out_pad, grad_pad, rope_grad,
+                                 torch.is_grad_enabled())
     if use_hip(qkv) and not sinks:
         if qkv.dtype == torch.bfloat16 and flash_supported(D, S):
             return _FlashPacked.apply(qkv, B, S, H, KV, D, causal, int(window or 0), scale, out_pad, grad_pad, docs,
