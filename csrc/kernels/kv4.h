@@ -64,20 +64,37 @@ DEV_INLINE uint32_t kv4_scale(uint32_t key, float* rinv) {
   *rinv = (dead || bad) ? 0.f : 1.0f / s;
   return dead ? 0u : bad ? 0x7fc0u : (__float_as_uint(s) >> 16);
 }
-// code + 8 in 0..15.  x and s have 8-bit significands, so x / s is a half integer or at least 2^-10 away from
-// one: the product with the rounded reciprocal (error under 2^-19) is first rounded to a multiple of 2^-11
-// (the add of 1.5 * 2^12), which puts it exactly on the ties it stands for and moves it over none; then
-// 1.5 * 2^23 + 8 rounds half to even and leaves the integer in the low bits.
+// code + 8 in 0..15, with 0x4b400000 on top.  x and s have 8-bit significands, so x / s is a half integer or at least
+// 2^-10 away from one: the product with the rounded reciprocal (error under 2^-19) is first rounded to a multiple of
+// 2^-11 (6144 = 1.5 * 2^12 is added), which puts it exactly on the ties it stands for and moves it over none; the second
+// sum, x / s + 1.5 * 2^23 + 8, rounds half to even and leaves the integer in the low bits.
 DEV_INLINE uint32_t kv4_code(float x, float rinv) {
-  const float t = (x * rinv + 6144.0f) - 6144.0f;
-  const uint32_t n = __float_as_uint(t + 12582920.0f) - 0x4b400000u;
-  return n < 15u ? n : 15u;
+  const uint32_t n = __float_as_uint((x * rinv + 6144.0f) + 12576776.0f);
+  return n < 0x4b40000fu ? n : 0x4b40000fu;
+}
+// Codes are packed by shift-and-add; the constants on top add up to a known sum that is taken off at the end.
+constexpr uint32_t kv4_top(int s0, int s1, int s2, int s3) {
+  return (0x4b400000u << s0) + (0x4b400000u << s1) + (0x4b400000u << s2) + (0x4b400000u << s3);
+}
+// 8 values of a K word: even d in the low half, odd d in the high half
+DEV_INLINE uint32_t kv4_pack_k(const float* f, float rinv) {
+  uint32_t w = 0u - kv4_top(0, 4, 8, 12) - kv4_top(16, 20, 24, 28);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) w += kv4_code(f[e], rinv) << (16 * (e & 1) + 4 * (e >> 1));
+  return w;
+}
+// 4 values of a V half word
+DEV_INLINE uint32_t kv4_pack_v(const float* f, float rinv) {
+  uint32_t w = 0u - kv4_top(0, 4, 8, 12);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) w += kv4_code(f[e], rinv) << (4 * e);
+  return w;  // (below 2^16: the tops cancel modulo 2^32)
 }
 
 // ---- one token's row, quantised by one wave: lanes 0..31 hold K, 32..63 V, 4 values from d = 4 (lane & 31) each
 // (D = 64: the first 16 of each half).  A group of 32 is 8 lanes: its maximum takes two quad permutes and a
 // mirror of 8.
-DEV_INLINE uint32_t kv4_dpp(uint32_t v, int ctrl_is) {
+DEV_INLINE uint32_t kv4_dpp(uint32_t v, int ctrl_is) {  // (a constant in every call)
   return ctrl_is == 1   ? (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xf, 0xf, true)   // lane ^ 1
          : ctrl_is == 2 ? (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xf, 0xf, true)   // lane ^ 2
                         : (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xf, 0xf, true);  // 7 - lane of 8
@@ -95,10 +112,10 @@ DEV_INLINE Kv4Token kv4_token(uint2 u, int lane) {
   float rinv;
   Kv4Token t;
   t.scale = kv4_scale(a > b ? a : b, &rinv);
-  const uint32_t n0 = kv4_code(bf_lo(u.x), rinv), n1 = kv4_code(bf_hi(u.x), rinv);
-  const uint32_t n2 = kv4_code(bf_lo(u.y), rinv), n3 = kv4_code(bf_hi(u.y), rinv);
-  const uint32_t kw = (n0 | n2 << 4 | n1 << 16 | n3 << 20) << (8 * (lane & 1));
-  t.code = lane < 32 ? (kw | kv4_dpp(kw, 1)) : (n0 | n1 << 4 | n2 << 8 | n3 << 12);
+  const float f[4] = {bf_lo(u.x), bf_hi(u.x), bf_lo(u.y), bf_hi(u.y)};
+  const uint32_t n = kv4_pack_v(f, rinv);  // nibbles d 0 1 2 3
+  const uint32_t kw = ((n & 0xfu) | (n & 0xf00u) >> 4 | (n & 0xf0u) << 12 | (n & 0xf000u) << 8) << (8 * (lane & 1));
+  t.code = lane < 32 ? (kw | kv4_dpp(kw, 1)) : n;
   return t;
 }
 template <int D>

@@ -21,8 +21,13 @@ struct StoreArgs {
   int B, KV, n, tiles, span;         // span: records a sequence's rows can touch
 };
 
-// 4-lane or 8-lane (lanes differing in the given xor masks) maximum of packed keys, both halves
-DEV_INLINE uint32_t key_max_x(uint32_t k, int m) { return kv4_max2(k, (uint32_t)__shfl_xor((int)k, m, 64)); }
+// maximum of packed keys (both halves) over lanes l, l ^ 16, l ^ 32, l ^ 48: row swaps, no LDS
+DEV_INLINE uint32_t key_max_q(uint32_t k) {
+  const auto a = __builtin_amdgcn_permlane16_swap(k, k, false, false);
+  k = kv4_max2(a[0], a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(k, k, false, false);
+  return kv4_max2(b[0], b[1]);
+}
 DEV_INLINE uint32_t key_top(uint32_t k) {
   const uint32_t a = k & 0xffffu, b = k >> 16;
   return a > b ? a : b;
@@ -35,11 +40,10 @@ template <int D>
 __global__ __launch_bounds__(256) void kv4_store_kernel(StoreArgs a) {
   using L = Kv4<D>;
   const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
-  const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const long long total = (long long)a.B * a.span * a.KV;
-  if (item >= total) return;
-  const int kvh = (int)(item % a.KV);
-  const int sp = (int)(item / a.KV % a.span), b = (int)(item / a.KV / a.span);
+  const unsigned item = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));  // < 2^31 (launcher)
+  if (item >= (unsigned)a.B * a.span * a.KV) return;
+  const int kvh = item % (unsigned)a.KV, bs = item / (unsigned)a.KV;
+  const int sp = bs % (unsigned)a.span, b = bs / (unsigned)a.span;
   const long long start = a.start[b];
   const int n = a.count ? min(a.n, a.count[b]) : a.n;
   // first record that the rows touch inside the cache (rows before position 0 are not written)
@@ -54,26 +58,47 @@ __global__ __launch_bounds__(256) void kv4_store_kernel(StoreArgs a) {
   const uint16_t* vp = a.v + b * a.v_bs + (long long)kvh * D;
   auto valid = [&](int t) { return row0 + t >= 0 && row0 + t < n; };
 
+  // every load of the record first: under per-row conditions and loops the compiler waits for each (rows that are not
+  // written are read as a row that is)
+  auto row_of = [&](int t) { return min(max(row0 + t, 0LL), (long long)n - 1); };
+  uint4 ku[2][L::NG];
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const uint16_t* p = kp + row_of(8 * (r >> 2) + 4 * half + (r & 3)) * a.k_rs + 8 * q;
+#pragma unroll
+    for (int j = 0; j < L::NG; ++j) ku[half][j] = *reinterpret_cast<const uint4*>(p + 32 * j);
+  }
+  uint4 vu[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint16_t* p = vp + row_of(8 * q + i) * a.v_rs + L::NJ * r;
+    if constexpr (D == 128) {
+      vu[i] = *reinterpret_cast<const uint4*>(p);
+    } else {
+      const uint2 u = *reinterpret_cast<const uint2*>(p);
+      vu[i] = make_uint4(u.x, u.y, 0, 0);
+    }
+  }
+
   // ---- K: this lane's token of each half, 8 values of every group
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
     const int t = 8 * (r >> 2) + 4 * half + (r & 3);
     const bool ok = whole || valid(t);
-    uint32_t w[L::NG];
+    uint32_t w[L::NG], sc[L::NG];
 #pragma unroll
     for (int j = 0; j < L::NG; ++j) {
-      uint4 u = make_uint4(0, 0, 0, 0);
-      if (ok) u = *reinterpret_cast<const uint4*>(kp + (row0 + t) * a.k_rs + 32 * j + 8 * q);
       float rinv, f[8];
-      const uint32_t s = kv4_scale(key_top(key_max_x(key_max_x(keys8(u), 16), 32)), &rinv);
-      unpack8(u, f);
-      w[j] = 0;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) w[j] |= kv4_code(f[e], rinv) << (16 * (e & 1) + 4 * (e >> 1));
-      if (ok && q == j)
-        *reinterpret_cast<uint16_t*>(rec + L::KS + ((r >> 2) * L::NG + j) * 16 + (4 * half + (r & 3)) * 2) = (uint16_t)s;
+      sc[j] = kv4_scale(key_top(key_max_q(keys8(ku[half][j]))), &rinv);
+      unpack8(ku[half][j], f);
+      w[j] = kv4_pack_k(f, rinv);
     }
     if (ok) {
+      uint32_t s = sc[0];  // lane q stores the scale of group q
+#pragma unroll
+      for (int j = 1; j < L::NG; ++j) s = q == j ? sc[j] : s;
+      if (q < L::NG)
+        *reinterpret_cast<uint16_t*>(rec + L::KS + ((r >> 2) * L::NG + q) * 16 + (4 * half + (r & 3)) * 2) = (uint16_t)s;
       if constexpr (D == 128)
         *reinterpret_cast<uint4*>(rec + L::KC + half * 1024 + lane * 16) = make_uint4(w[0], w[1], w[2], w[3]);
       else
@@ -91,25 +116,15 @@ __global__ __launch_bounds__(256) void kv4_store_kernel(StoreArgs a) {
   }
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const bool ok = whole || valid(8 * q + i);
     float f[8], rinv;
-    uint32_t key;
-    if constexpr (D == 128) {
-      uint4 u = make_uint4(0, 0, 0, 0);
-      if (ok) u = *reinterpret_cast<const uint4*>(vp + (row0 + 8 * q + i) * a.v_rs + 8 * r);
-      key = keys8(u);
-      unpack8(u, f);
-    } else {
-      uint2 u = make_uint2(0, 0);
-      if (ok) u = *reinterpret_cast<const uint2*>(vp + (row0 + 8 * q + i) * a.v_rs + 4 * r);
-      key = kv4_max2(kv4_keys(u.x), kv4_keys(u.y));
-      f[0] = bf_lo(u.x); f[1] = bf_hi(u.x); f[2] = bf_lo(u.y); f[3] = bf_hi(u.y);
-    }
-    key = key_max_x(key_max_x(key, 1), 2);
-    if constexpr (D == 64) key = key_max_x(key, 4);
+    uint32_t key = keys8(vu[i]);  // (the zeros past 4 values at D = 64 raise no maximum)
+    unpack8(vu[i], f);
+    key = kv4_max2(key, kv4_dpp(key, 1));
+    key = kv4_max2(key, kv4_dpp(key, 2));
+    if constexpr (D == 64) key = kv4_max2(key, kv4_dpp(key, 3));
     sc[i >> 1] |= kv4_scale(key_top(key), &rinv) << (16 * (i & 1));
 #pragma unroll
-    for (int e = 0; e < L::NJ; ++e) w[e >> 2][i >> 1] |= kv4_code(f[e], rinv) << (16 * (i & 1) + 4 * (e & 3));
+    for (int c = 0; c < L::CH; ++c) w[c][i >> 1] |= kv4_pack_v(f + 4 * c, rinv) << (16 * (i & 1));
   }
   constexpr int LPG = 16 / L::NG;  // lanes r per group
   if (whole) {
@@ -137,10 +152,10 @@ template <int D>
 __global__ __launch_bounds__(256) void kv4_store_token_kernel(StoreArgs a) {
   using L = Kv4<D>;
   const int lane = threadIdx.x & 63;
-  const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (item >= (long long)a.B * a.n * a.KV) return;
-  const int kvh = (int)(item % a.KV);
-  const int i = (int)(item / a.KV % a.n), b = (int)(item / a.KV / a.n);
+  const unsigned item = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+  if (item >= (unsigned)a.B * a.n * a.KV) return;
+  const int kvh = item % (unsigned)a.KV, bi = item / (unsigned)a.KV;
+  const int i = bi % (unsigned)a.n, b = bi / (unsigned)a.n;
   const int d = (4 * (lane & 31)) % D;
   const uint16_t* p = (lane < 32 ? a.k + b * a.k_bs + i * a.k_rs : a.v + b * a.v_bs + i * a.v_rs) + (long long)kvh * D + d;
   const uint2 u = *reinterpret_cast<const uint2*>(p);
@@ -163,11 +178,10 @@ template <int D>
 __global__ __launch_bounds__(256) void kv4_load_kernel(LoadArgs a) {
   using L = Kv4<D>;
   const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
-  const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const long long total = (long long)a.B * a.span * a.KV;
-  if (item >= total) return;
-  const int kvh = (int)(item % a.KV);
-  const int sp = (int)(item / a.KV % a.span), b = (int)(item / a.KV / a.span);
+  const unsigned item = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));  // < 2^31 (launcher)
+  if (item >= (unsigned)a.B * a.span * a.KV) return;
+  const int kvh = item % (unsigned)a.KV, bs = item / (unsigned)a.KV;
+  const int sp = bs % (unsigned)a.span, b = bs / (unsigned)a.span;
   const long long start = a.start[b];
   const long long tile = (start >= 0 ? start / KV4_TILE : -((-start + KV4_TILE - 1) / KV4_TILE)) + sp;
   const long long row0 = tile * KV4_TILE - start;
@@ -179,29 +193,32 @@ __global__ __launch_bounds__(256) void kv4_load_kernel(LoadArgs a) {
   uint16_t* vp = a.v + (long long)b * a.n * W + (long long)kvh * D;
   auto valid = [&](int t) { return row0 + t >= 0 && row0 + t < a.n; };
 
+  // K: whole rows per store instruction (16 bytes a lane), from 4-byte reads of the record: 5.3 TB/s of record and row
+  // bytes at 64 x 2048 tokens of 8 heads x 128, 3.9 where each lane writes out its own chunk (64-byte pieces)
+  constexpr int CPR = D / 8, RPI = 64 / CPR;  // 16-byte pieces a row, rows an instruction
+  uint32_t kw[32 / RPI];
+  float ks[32 / RPI];
+  const int kc = lane % CPR;
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    const int t = 8 * (r >> 2) + 4 * half + (r & 3);
-    if (!valid(t)) continue;
-    uint32_t w[L::NG];
-#pragma unroll
-    for (int j = 0; j < L::NG; ++j)
-      w[j] = *reinterpret_cast<const uint32_t*>(rec + L::KC + (D == 128 ? half * 1024 + lane * 16 : lane * 16 + half * 8) + 4 * j);
-#pragma unroll
-    for (int j = 0; j < L::NG; ++j) {
-      const float s = bf2f(*reinterpret_cast<const uint16_t*>(rec + L::KS + ((r >> 2) * L::NG + j) * 16 + (4 * half + (r & 3)) * 2));
-      float f[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] = s * ((float)(int)((w[j] >> (16 * (e & 1) + 4 * (e >> 1))) & 15u) - 8.0f);
-      const uint4 u = in ? pack8(f) : make_uint4(0, 0, 0, 0);
-      *reinterpret_cast<uint4*>(kp + (row0 + t) * W + 32 * j + 8 * q) = u;
-    }
+  for (int i = 0; i < 32 / RPI; ++i) {
+    int off, sh, so;
+    L::k_at(i * RPI + lane / CPR, 8 * kc, &off, &sh, &so);
+    kw[i] = *reinterpret_cast<const uint32_t*>(rec + off);
+    ks[i] = bf2f(*reinterpret_cast<const uint16_t*>(rec + so));
   }
   constexpr int LPG = 16 / L::NG;
   uint4 w[L::CH];
 #pragma unroll
   for (int c = 0; c < L::CH; ++c) w[c] = *reinterpret_cast<const uint4*>(rec + L::VC + c * 1024 + lane * 16);
   const uint4 sc = *reinterpret_cast<const uint4*>(rec + L::VS + (q * L::NG + r / LPG) * 16);
+#pragma unroll
+  for (int i = 0; i < 32 / RPI; ++i) {
+    const int t = i * RPI + lane / CPR;
+    float f[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = ks[i] * ((float)(int)((kw[i] >> (16 * (e & 1) + 4 * (e >> 1))) & 15u) - 8.0f);
+    if (valid(t)) *reinterpret_cast<uint4*>(kp + (row0 + t) * W + 8 * kc) = in ? pack8(f) : make_uint4(0, 0, 0, 0);
+  }
   float s[8];
   unpack8(sc, s);
 #pragma unroll
@@ -237,7 +254,7 @@ extern "C" int ftc_kv4_store(void* data, const void* k, const void* v, const int
   const int span = kv4_span(n);
   const bool tokens = n < KV4_STORE_TOKENS;
   const long long blocks = ((long long)B * KV * (tokens ? n : span) + 3) / 4;
-  if (blocks > 0x7fffffffLL) return -1;
+  if (blocks > 0x1fffffffLL) return -1;  // a wave's index stays below 2^31
   StoreArgs a{(uint8_t*)data, (const uint16_t*)k, (const uint16_t*)v, start, count, k_bs, k_rs, v_bs, v_rs,
               B, KV, n, tiles, span};
   if (tokens && D == 128)
@@ -256,7 +273,7 @@ extern "C" int ftc_kv4_load(const void* data, void* k, void* v, const int* start
   if ((D != 64 && D != 128) || B < 1 || KV < 1 || n < 1 || tiles < 1) return -1;
   const int span = kv4_span(n);
   const long long blocks = ((long long)B * KV * span + 3) / 4;
-  if (blocks > 0x7fffffffLL) return -1;
+  if (blocks > 0x1fffffffLL) return -1;  // a wave's index stays below 2^31
   LoadArgs a{(const uint8_t*)data, (uint16_t*)k, (uint16_t*)v, start, B, KV, n, tiles, span};
   if (D == 128)
     hipLaunchKernelGGL(kv4_load_kernel<128>, dim3((unsigned)blocks), dim3(256), 0, stream, a);

@@ -59,8 +59,8 @@ def test_quantisation_matches_the_exact_definition(kind):
 
 
 def test_kernel_rounding_is_exact_for_every_pair_of_significands():
-    """The kernel forms x / s as a product with the rounded reciprocal, snaps it to multiples of 2^-11 and adds
-    1.5 * 2^23 + 8 (kv4.h kv4_code).  The same arithmetic in numpy against exact integers, for every significand of
+    """The kernel forms x / s as a product with the rounded reciprocal, snaps it to multiples of 2^-11 (the sum
+    with 6144) and rounds the sum with 1.5 * 2^23 + 8 (kv4.h kv4_code).  The same arithmetic in numpy against exact integers, for every significand of
     x and s at every exponent distance that gives |x / s| <= 8."""
     f32 = np.float32
     X = np.arange(128, 256, dtype=np.int64)[:, None]
@@ -71,8 +71,7 @@ def test_kernel_rounding_is_exact_for_every_pair_of_significands():
         for fused in (False, True):  # the compiler may contract the product into the add
             prod = x.astype(np.float64) * rinv.astype(np.float64)
             t = (prod + 6144.0).astype(f32) if fused else (prod.astype(f32) + f32(6144.0))
-            t = (t - f32(6144.0)).astype(f32)
-            n = (t + f32(12582920.0)).astype(f32).view(np.int32) - 0x4B400000
+            n = (t + f32(12576776.0)).astype(f32).view(np.int32) - 0x4B400000
             num, den = X * (1 << (k + 12)), S * (1 << 12)
             q, r = num // den, num % den
             want = q + ((2 * r > den) | ((2 * r == den) & (q % 2 == 1)))
