@@ -288,6 +288,10 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void sink_fwd_kernel(FwdArgs
   // wave passed this tile's barrier
   auto tile = [&](const int t, const char* Kc, const char* Vc, char* Kn, char* Vn) __attribute__((always_inline)) {
     sync_tile(t, Kn, Vn);
+    // a wave sees nothing of the tiles past its rows and before its window: with a short window they are many (341 us
+    // instead of 362 at 4 x 4096 tokens, window 1024, 32 heads x 128; 0-1 % at 4096 of 8192 and 16384)
+    const int kv0 = tile_key(t), qw = q0 + wave * 32;
+    if (kv0 > qw + 31 || (qw - (kv0 + BK - 1) >= a.window && kv0 >= a.sinks)) return;
     phaseA(Kc);
     phaseB1(t);
     phaseB2(Vc);
@@ -373,6 +377,8 @@ struct BwdArgs {
   int window, sinks;
   float* far;  // [B * KV, nfar, sinks, 2 (dK before the scale, dV), D] sums of the sink keys' far queries (null: none)
   int nfar;
+  float* ksum;  // [B * KV, kparts, S, 2, D] sums of key blocks swept in parts (kparts > 1)
+  int kparts;
   const float* rcos;  // RoPE folded into the dQ / dK epilogues (rope_inv_rows), or null
   const float* rsin;
   const int* rpos;
@@ -380,7 +386,8 @@ struct BwdArgs {
 
 // ---------------------------------------------------------------- dK / dV
 // As bwd_dkdv8_kernel (8 waves x 32 keys in ping-pong phase order, 5-slot DMA ring), windowed.
-template <int D, int QR>
+// PARTS: the workgroup sweeps one part of the block's slices and leaves 32-bit sums for sink_join_kernel.
+template <int D, int QR, bool PARTS>
 __global__ __launch_bounds__(512, 1) void sink_dkdv_kernel(BwdArgs a) {
   constexpr int DIST = 3;
   static_assert(QR == 1 || QR == 2, "one or two 32-row query blocks per slice");
@@ -405,8 +412,9 @@ __global__ __launch_bounds__(512, 1) void sink_dkdv_kernel(BwdArgs a) {
   const int S = a.S, G = a.H / a.KV;
   const int npairs = a.B * a.KV;
   int kb, pair;
+  const int part = PARTS ? blockIdx.x % a.kparts : 0;
   {
-    const int bid = blockIdx.x;
+    const int bid = PARTS ? blockIdx.x / a.kparts : blockIdx.x;
     if ((npairs & 7) == 0) {
       const int xcd = bid & 7, slot = bid >> 3, ppx = npairs >> 3;
       kb = slot / ppx;
@@ -448,6 +456,8 @@ __global__ __launch_bounds__(512, 1) void sink_dkdv_kernel(BwdArgs a) {
   // queries whose window reaches this key block (the sink keys' later queries: sink_far_kernel)
   const int qbeg = kv0 / BQ2 * BQ2, qend = min(S, kv0 + BKV - 1 + a.window);
   const int nqt = (qend - qbeg + BQ2 - 1) / BQ2;
+  const int per = PARTS ? (G * nqt + a.kparts - 1) / a.kparts : G * nqt, it0 = part * per;
+  const int total = PARTS ? min(per, G * nqt - it0) : per;
   // Q / dO / row-constant slices arrive by LDS-DMA (global_load_lds_dwordx4: no staging VGPRs) into a
   // 5-slot ring, three slices ahead of the compute; one raw barrier per slice with a COUNTED vmcnt so the
   // next slice's DMA stays in flight across it.  The swizzled
@@ -475,7 +485,7 @@ __global__ __launch_bounds__(512, 1) void sink_dkdv_kernel(BwdArgs a) {
   // QR = 1: lanes 0..31 -lse/scale of the 32 rows, lanes 32..63 -delta (every wave issues the same
   // piece); QR = 2: one piece of the 64 rows' -lse/scale and one of their -delta
   auto issue = [&](int it_, char* base_) {
-    const int g_ = it_ / nqt, qt_ = qbeg + (it_ % nqt) * BQ2;
+    const int g_ = (it0 + it_) / nqt, qt_ = qbeg + ((it0 + it_) % nqt) * BQ2;
     const int hq_ = kvh * G + g_, left = S - 1 - qt_;
     int qvo[NG], dvo[NG];
 #pragma unroll
@@ -493,7 +503,6 @@ __global__ __launch_bounds__(512, 1) void sink_dkdv_kernel(BwdArgs a) {
   constexpr int VM_ZERO = 0x0F70;                                               // vmcnt(0)
   constexpr int LGKM_ZERO = 0xC07F;                                             // lgkmcnt(0)
 
-  const int total = G * nqt;
   // K staging and the V fragments are ordinary loads: retire them before the first DMA so no
   // compiler-inserted wait inside the loop has to count them
   __builtin_amdgcn_s_waitcnt(VM_ZERO);
@@ -555,7 +564,7 @@ __global__ __launch_bounds__(512, 1) void sink_dkdv_kernel(BwdArgs a) {
   auto phaseB1 = [&](const int it) __attribute__((always_inline)) {
 #pragma unroll
     for (int r = 0; r < QR; ++r) {
-      const int qt = qbeg + (it % nqt) * BQ2 + 32 * r;
+      const int qt = qbeg + ((it0 + it) % nqt) * BQ2 + 32 * r;
       const int key = wkey0 + lr;
       const bool need_mask = qt < wkey0 + 31 || qt + 31 - wkey0 >= a.window || qt + 32 > S;
 #pragma unroll
@@ -596,6 +605,14 @@ __global__ __launch_bounds__(512, 1) void sink_dkdv_kernel(BwdArgs a) {
       }
     }
   };
+  // some key of this wave is seen by some query of the slice (the others are skipped: backward 1113 instead of 1151 us at
+  // 4 x 4096 tokens, window 1024; 741 instead of 798 at 2 x 8192, window 512; 1 % slower at 8192, window 4096); not in
+  // parts, whose kernel would spill 374 registers for it
+  auto seen = [&](const int it) __attribute__((always_inline)) {
+    if constexpr (PARTS) return true;
+    const int qt = qbeg + ((it0 + it) % nqt) * BQ2;
+    return qt + BQ2 - 1 >= wkey0 && qt - (wkey0 + 31) < a.window;
+  };
   // one barrier per slice: slice it is in LDS for every wave, the DMA of slice it + 2 goes out
   auto sync_slice = [&](const int it, char* dma_slot) __attribute__((always_inline)) {
     if (it + 2 < total) {
@@ -618,6 +635,7 @@ __global__ __launch_bounds__(512, 1) void sink_dkdv_kernel(BwdArgs a) {
   if (wave < 4) {  // waves w and w + 4 share a SIMD
     auto body = [&](const int it, const char* Qs, char* dma_slot) __attribute__((always_inline)) {
       sync_slice(it, dma_slot);
+      if (!seen(it)) return;
       phaseA(Qs);
       phaseB1(it);
       phaseB2(Qs);
@@ -632,7 +650,8 @@ __global__ __launch_bounds__(512, 1) void sink_dkdv_kernel(BwdArgs a) {
   } else {
     auto body = [&](const int it, const char* Qs, const char* Qprev, char* dma_slot) __attribute__((always_inline)) {
       sync_slice(it, dma_slot);
-      if (it > 0) phaseB2(Qprev);
+      if (it > 0 && seen(it - 1)) phaseB2(Qprev);
+      if (!seen(it)) return;
       phaseA(Qs);
       phaseB1(it);
     };
@@ -643,7 +662,7 @@ __global__ __launch_bounds__(512, 1) void sink_dkdv_kernel(BwdArgs a) {
       if (it + 3 < total) body(it + 3, slot3, slot2, slot1);
       if (it + 4 < total) body(it + 4, slot4, slot3, slot2);
     }
-    if (total > 0) {
+    if (total > 0 && seen(total - 1)) {
       const int r = (total - 1) % 5;
       phaseB2(r == 0 ? slot0 : r == 1 ? slot1 : r == 2 ? slot2 : r == 3 ? slot3 : slot4);
     }
@@ -652,6 +671,19 @@ __global__ __launch_bounds__(512, 1) void sink_dkdv_kernel(BwdArgs a) {
   // ---- epilogue: dK = scale * dK^T^T, dV; lane owns one key row
   const int key = wkey0 + lr;
   if (key >= S) return;
+  if constexpr (PARTS) {
+    float* p = a.ksum + (((long long)pair * a.kparts + part) * S + key) * 2 * D + 4 * hh;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int g4 = 0; g4 < 4; ++g4) {
+        *reinterpret_cast<float4*>(p + 32 * dt + 8 * g4) =
+            make_float4(dk[dt][4 * g4], dk[dt][4 * g4 + 1], dk[dt][4 * g4 + 2], dk[dt][4 * g4 + 3]);
+        *reinterpret_cast<float4*>(p + D + 32 * dt + 8 * g4) =
+            make_float4(dv[dt][4 * g4], dv[dt][4 * g4 + 1], dv[dt][4 * g4 + 2], dv[dt][4 * g4 + 3]);
+      }
+    return;
+  }
   if (a.far && key < a.sinks) {  // queries past this key's window
     const float* fp = a.far + ((long long)pair * a.nfar * a.sinks + key) * 2 * D + 4 * hh;
     for (int n = 0; n < a.nfar; ++n, fp += (long long)a.sinks * 2 * D) {
@@ -674,6 +706,55 @@ __global__ __launch_bounds__(512, 1) void sink_dkdv_kernel(BwdArgs a) {
   }
   store_rows<DT>(dkp, dk, a.scale, hh, wide);
   store_rows<DT>(dvp, dv, 1.0f, hh, wide);
+}
+
+// dK / dV rows of key blocks that were swept in parts: the parts' sums and the sink keys' far sums in order, then the
+// same epilogue.  A thread holds 4 columns of each half of a row (RoPE pairs d with d + 64).
+template <int D>
+__global__ __launch_bounds__(256) void sink_join_kernel(BwdArgs a) {
+  constexpr int TPK = D / 8;  // threads a key
+  const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
+  const long long row = id / TPK;  // pair * S + key
+  const int d0 = (int)(id % TPK) * 4;
+  if (row >= (long long)a.B * a.KV * a.S) return;
+  const int key = (int)(row % a.S), pair = (int)(row / a.S), kvh = pair % a.KV, b = pair / a.KV;
+  float acc[2][2][4] = {};  // dK | dV, halves of the row
+  auto add = [&](const float* p) __attribute__((always_inline)) {
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float4 x = *reinterpret_cast<const float4*>(p + m * D + h * (D / 2) + d0);
+        acc[m][h][0] += x.x; acc[m][h][1] += x.y; acc[m][h][2] += x.z; acc[m][h][3] += x.w;
+      }
+  };
+#pragma unroll 4
+  for (int n = 0; n < a.kparts; ++n) add(a.ksum + (((long long)pair * a.kparts + n) * a.S + key) * 2 * D);
+  if (a.far && key < a.sinks) {
+#pragma unroll 4
+    for (int n = 0; n < a.nfar; ++n) add(a.far + (((long long)pair * a.nfar + n) * a.sinks + key) * 2 * D);
+  }
+  const long long token = (long long)b * a.S + key;
+  if constexpr (D == 128) {
+    if (a.rcos) {
+      const long long t = (long long)(a.rpos ? a.rpos[token] : key) * 64 + d0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float c = a.rcos[t + e], sn = a.rsin[t + e], g1 = acc[0][0][e], g2 = acc[0][1][e];
+        acc[0][0][e] = g1 * c + g2 * sn;
+        acc[0][1][e] = g2 * c - g1 * sn;
+      }
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    uint16_t* o = (m ? a.dv : a.dk) + token * a.dkv_rs + (long long)kvh * D + d0;
+    const float sc = m ? 1.0f : a.scale;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      *reinterpret_cast<uint2*>(o + h * (D / 2)) = make_uint2(pack_bf2(acc[m][h][0] * sc, acc[m][h][1] * sc),
+                                                              pack_bf2(acc[m][h][2] * sc, acc[m][h][3] * sc));
+  }
 }
 
 // ---------------------------------------------------------------- dK / dV of the sink keys, far queries
@@ -1024,10 +1105,33 @@ static int far_parts(int B, int S, int H, int KV, int window, int sinks) {
   return (int)(r < 1 ? 1 : r);
 }
 
-// floats: [-delta | -lse/scale], then the far sums
+// Parts that a key block's sweep is split into where there are few blocks: one workgroup a CU, at least 4 slices a part.
+// Measured against 1 to 32 parts (whole backward): 1 x 2048 tokens, 32 / 8 heads x 128, window 512 (64 blocks): 4 parts
+// 139 us, 3 145, 6 168, unsplit 247; 1 x 4096, window 1024 (128 blocks): 2 parts 310, 3 366, unsplit 438; 1 x 1001, 8 / 2
+// heads, window 256 (8 blocks): 16 parts 62, 32 64, unsplit 146; 144 blocks: 2 parts 59, unsplit 53.
+static int key_parts(int B, int S, int H, int KV, int D, int window) {
+  const long long blocks = (long long)B * KV * ((S + 255) / 256);
+  const int rows = D == 128 ? 32 : 64;  // a slice
+  const long long span = 255LL + window < S ? 255 + window : S, slices = (span + rows - 1) / rows * (H / KV);
+  const long long p = 256 / blocks, most = slices / 4, r = p < most ? p : most;
+  return (int)(r < 1 ? 1 : r);
+}
+struct Ws {
+  int nfar, kparts;
+  long long far, ksum, total;  // floats: [-delta | -lse/scale], far sums, part sums
+};
+static Ws bwd_ws(int B, int S, int H, int KV, int D, int window, int sinks) {
+  Ws w;
+  const long long n = sinks < S ? sinks : S;
+  w.nfar = far_parts(B, S, H, KV, window, sinks);
+  w.kparts = key_parts(B, S, H, KV, D, window);
+  w.far = (2LL * B * H * S + 3) / 4 * 4;
+  w.ksum = w.far + (long long)B * KV * w.nfar * n * 2 * D;
+  w.total = w.ksum + (w.kparts > 1 ? (long long)B * KV * w.kparts * S * 2 * D : 0);
+  return w;
+}
 extern "C" long long ftc_sink_bwd_workspace(int B, int S, int H, int KV, int D, int window, int sinks) {
-  const long long base = (2LL * B * H * S + 3) / 4 * 4, n = sinks < S ? sinks : S;
-  return base + (long long)B * KV * far_parts(B, S, H, KV, window, sinks) * n * 2 * D;
+  return bwd_ws(B, S, H, KV, D, window, sinks).total;
 }
 
 extern "C" int ftc_sink_bwd(const void* q, const void* k, const void* v, const void* o, const void* olow, const void* dout,
@@ -1042,22 +1146,34 @@ extern "C" int ftc_sink_bwd(const void* q, const void* k, const void* v, const v
   // one batch's Q / dO / K / V rows and the row constants are addressed with 32-bit buffer offsets
   const long long max_rs = q_rs > do_rs ? (q_rs > kv_rs ? q_rs : kv_rs) : (do_rs > kv_rs ? do_rs : kv_rs);
   if ((long long)S * max_rs * 2 >= (1LL << 31) || 2LL * B * H * S * 4 >= (1LL << 31)) return -1;
-  const int nfar = far_parts(B, S, H, KV, window, sinks);
+  const Ws w = bwd_ws(B, S, H, KV, D, window, sinks);
+  const int nfar = w.nfar;
   BwdArgs a{(const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, (const uint16_t*)o, (const uint16_t*)dout,
             (const uint8_t*)olow, lse, workspace, (uint16_t*)dq, (uint16_t*)dk, (uint16_t*)dv, q_rs, kv_rs, o_rs, dq_rs, dkv_rs, do_rs,
             B, S, H, KV, scale, scale * LOG2E, window < S ? window : S, sinks < S ? sinks : S,
-            nfar ? workspace + (2LL * B * H * S + 3) / 4 * 4 : nullptr, nfar, rope_cos, rope_sin, rope_pos};
-  const dim3 g_kv(B * KV * ((S + 255) / 256)), g_q(B * H * ((S + 127) / 128));
+            nfar ? workspace + w.far : nullptr, nfar, workspace + w.ksum, w.kparts, rope_cos, rope_sin, rope_pos};
+  const dim3 g_kv(B * KV * ((S + 255) / 256) * w.kparts), g_q(B * H * ((S + 127) / 128));
   const dim3 g_far(B * KV * nfar * ((a.sinks + 31) / 32));
+  const dim3 g_join((unsigned)(((long long)B * KV * S * (D / 8) + 255) / 256));
   // dQ first: it writes the row constants that the other two read
   if (D == 128) {
     hipLaunchKernelGGL((sink_dq_kernel<128>), g_q, dim3(256), 0, stream, a);
     if (nfar) hipLaunchKernelGGL((sink_far_kernel<128>), g_far, dim3(64 * FAR_WAVES), 0, stream, a);
-    hipLaunchKernelGGL((sink_dkdv_kernel<128, 1>), g_kv, dim3(512), 0, stream, a);
+    if (w.kparts > 1) {
+      hipLaunchKernelGGL((sink_dkdv_kernel<128, 1, true>), g_kv, dim3(512), 0, stream, a);
+      hipLaunchKernelGGL((sink_join_kernel<128>), g_join, dim3(256), 0, stream, a);
+    } else {
+      hipLaunchKernelGGL((sink_dkdv_kernel<128, 1, false>), g_kv, dim3(512), 0, stream, a);
+    }
   } else {
     hipLaunchKernelGGL((sink_dq_kernel<64>), g_q, dim3(256), 0, stream, a);
     if (nfar) hipLaunchKernelGGL((sink_far_kernel<64>), g_far, dim3(64 * FAR_WAVES), 0, stream, a);
-    hipLaunchKernelGGL((sink_dkdv_kernel<64, 2>), g_kv, dim3(512), 0, stream, a);
+    if (w.kparts > 1) {
+      hipLaunchKernelGGL((sink_dkdv_kernel<64, 2, true>), g_kv, dim3(512), 0, stream, a);
+      hipLaunchKernelGGL((sink_join_kernel<64>), g_join, dim3(256), 0, stream, a);
+    } else {
+      hipLaunchKernelGGL((sink_dkdv_kernel<64, 2, false>), g_kv, dim3(512), 0, stream, a);
+    }
   }
   return (int)hipGetLastError();
 }

@@ -111,6 +111,9 @@ SHAPES = [  # B, S, H, KV, D, window, sinks
     (1, 1300, 2, 2, 128, 40, 260),
     (1, 600, 6, 3, 80, 50, 5),
     (2, 77, 2, 1, 32, 9, 2),
+    (1, 700, 8, 1, 128, 200, 40),  # few key blocks: swept in parts
+    (2, 530, 4, 2, 64, 530, 3),
+    (16, 260, 32, 16, 64, 100, 5),  # many: each by one workgroup
 ]
 
 
