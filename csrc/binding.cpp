@@ -53,7 +53,7 @@ long long ftc_decode_workspace_floats(int B, int H, int KV, int D, int max_len);
 int ftc_decode_attention(const void* q, void* kc, void* vc, const void* knew, const void* vnew, long long new_rs,
                          const int* lens, void* out, float* workspace, int B, int H, int KV, int D, int max_len,
                          long long q_rs, long long kv_rs, long long b_rs, long long o_rs, float scale, int window,
-                         hipStream_t stream);
+                         int sinks, hipStream_t stream);
 int ftc_flash_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, const float* lse,
                   void* dq, void* dk, void* dv, void* workspace, int B, int S, int H, int KV, int D,
                   long long q_row_stride, long long kv_row_stride, long long o_row_stride, long long do_row_stride,
@@ -639,7 +639,8 @@ at::Tensor sink_bwd(const at::Tensor& qkv, const at::Tensor& o, const at::Tensor
 // <= Lmax).  The current token's K/V rows are appended at position lens-1 by the kernel itself.
 at::Tensor decode_attention(const at::Tensor& q, at::Tensor& k_cache, at::Tensor& v_cache,
                             const at::Tensor& lens, int64_t H, int64_t KV, int64_t D, int64_t max_len, double scale,
-                            int64_t window) {
+                            int64_t window, int64_t sinks) {
+  TORCH_CHECK(sinks >= 0, "decode_attention: sinks must not be negative");
   need(q, at::kBFloat16, "q");
   need(k_cache, at::kBFloat16, "k_cache");
   need(v_cache, at::kBFloat16, "v_cache");
@@ -661,7 +662,7 @@ at::Tensor decode_attention(const at::Tensor& q, at::Tensor& k_cache, at::Tensor
                              lens.data_ptr<int>(), out.data_ptr(), ws.data_ptr<float>(), (int)B, (int)H, (int)KV,
                              (int)D, (int)max_len,
                              q.stride(0), KV * D, Lmax * KV * D, out.stride(0), (float)scale, (int)window,
-                             cur_stream()),
+                             (int)std::min<int64_t>(sinks, 1 << 30), cur_stream()),
         "decode_attention");
   return out;
 }
@@ -972,7 +973,9 @@ PYBIND11_MODULE(_C, m) {
         py::arg("rope_cos") = py::none(), py::arg("rope_sin") = py::none(), py::arg("rope_pos") = py::none());
   m.def("sink_fwd", &sink_fwd);
   m.def("sink_bwd", &sink_bwd);
-  m.def("decode_attention", &decode_attention);
+  m.def("decode_attention", &decode_attention, py::arg("qkv"), py::arg("k_cache"), py::arg("v_cache"), py::arg("lens"),
+        py::arg("H"), py::arg("KV"), py::arg("D"), py::arg("max_len"), py::arg("scale"), py::arg("window"),
+        py::arg("sinks") = 0);
   m.def("kv4_store_", &kv4_store_);
   m.def("kv4_load", &kv4_load);
   m.def("decode_attention_kv4", &decode_attention_kv4);

@@ -1,5 +1,5 @@
 // Decode attention for generation: one new query token per sequence against its KV cache (GQA,
-// optional sliding window), split over the key axis so a batch of long caches fills the 256 CUs.
+// optional sliding window and sinks: the first keys stay visible), split over the key axis so a batch of long caches fills the 256 CUs.
 //
 // Decode is bound by HBM (every cached K/V byte is read once per generated token), so the layout is
 // chosen for coalesced 16-byte loads, not for MFMA:
@@ -38,7 +38,7 @@ struct DecArgs {
   float* ml;     // [B*H, nsplit, 2]
   uint16_t* out;
   long long q_rs, kv_rs, b_rs, o_rs, new_rs;
-  int B, H, KV, nsplit, window, chunk;
+  int B, H, KV, nsplit, window, chunk, sinks;
   float c;  // scale * log2(e)
 };
 
@@ -59,7 +59,7 @@ __global__ __launch_bounds__(256) void decode_partial_kernel(DecArgs a) {
   const int lo = a.window > 0 ? max(0, len - a.window) : 0;
   const int chunk = a.chunk, iters = chunk / (4 * KPW);
   const int k0 = split * chunk;
-  if (k0 >= len || k0 + chunk <= lo) return;  // the combine kernel skips this chunk too
+  if (k0 >= len || (k0 + chunk <= lo && k0 >= a.sinks)) return;  // the combine kernel skips this chunk too
   const int cur = len - 1;  // the current token: K / V from the projection output
 
   // the lane's 8-element slice of each query head of the group, pre-scaled into the log2 domain
@@ -81,7 +81,7 @@ __global__ __launch_bounds__(256) void decode_partial_kernel(DecArgs a) {
   for (int it = 0; it < iters; ++it) {
     const int kl = (it * 4 + wave) * KPW + kq;  // key within the chunk
     const int key = k0 + kl;
-    const bool ok = key >= lo && key < len;
+    const bool ok = (key >= lo || key < a.sinks) && key < len;
     float kf[8];
     uint4 u = make_uint4(0, 0, 0, 0);
     if (key == cur) {  // append the new row while using it
@@ -140,7 +140,7 @@ __global__ __launch_bounds__(256) void decode_partial_kernel(DecArgs a) {
   for (int it = 0; it < iters; ++it) {
     const int kl = (it * 4 + wave) * KPW + kq;
     const int key = k0 + kl;
-    const bool ok = key >= lo && key < len;
+    const bool ok = (key >= lo || key < a.sinks) && key < len;
     float vf[8];
     uint4 u = make_uint4(0, 0, 0, 0);
     if (key == cur) {
@@ -195,12 +195,16 @@ __global__ __launch_bounds__(D) void decode_combine_kernel(DecArgs a) {
   const int b = bh / a.H;
   const int len = a.lens[b];
   const int lo = a.window > 0 ? max(0, len - a.window) : 0;
+  // the chunks that hold sink keys, then those from the window's first
   const int s0 = lo / a.chunk, s1 = min(a.nsplit, (len + a.chunk - 1) / a.chunk);
+  const int ns = min((min(a.sinks, lo) + a.chunk - 1) / a.chunk, s0);
   const long long base = (long long)bh * a.nsplit;
   float M = -INFINITY;
+  for (int s = 0; s < ns; ++s) M = fmaxf(M, a.ml[(base + s) * 2]);
   for (int s = s0; s < s1; ++s) M = fmaxf(M, a.ml[(base + s) * 2]);
   float L = 0.f, o = 0.f;
-  for (int s = s0; s < s1; ++s) {
+  for (int i = s0 - ns; i < s1; ++i) {
+    const int s = i < s0 ? i - (s0 - ns) : i;
     const float w = __builtin_amdgcn_exp2f(a.ml[(base + s) * 2] - M);
     L += w * a.ml[(base + s) * 2 + 1];
     o += w * a.opart[(base + s) * D + d];
@@ -227,13 +231,13 @@ extern "C" long long ftc_decode_workspace_floats(int B, int H, int KV, int D, in
 extern "C" int ftc_decode_attention(const void* q, void* kc, void* vc, const void* knew, const void* vnew,
                                     long long new_rs, const int* lens, void* out, float* workspace, int B, int H,
                                     int KV, int D, int max_len, long long q_rs, long long kv_rs, long long b_rs,
-                                    long long o_rs, float scale, int window, hipStream_t stream) {
-  if ((D != 128 && D != 64) || H % KV != 0 || H / KV > GMAX || max_len < 1) return -1;
+                                    long long o_rs, float scale, int window, int sinks, hipStream_t stream) {
+  if (sinks < 0 || (D != 128 && D != 64) || H % KV != 0 || H / KV > GMAX || max_len < 1) return -1;
   const int chunk = decode_chunk(B, KV, max_len);
   const int nsplit = (max_len + chunk - 1) / chunk;
   DecArgs a{(const uint16_t*)q, (uint16_t*)kc, (uint16_t*)vc, (const uint16_t*)knew, (const uint16_t*)vnew, lens,
             workspace, workspace + (long long)B * H * nsplit * D, (uint16_t*)out,
-            q_rs, kv_rs, b_rs, o_rs, new_rs, B, H, KV, nsplit, window, chunk, scale * LOG2E};
+            q_rs, kv_rs, b_rs, o_rs, new_rs, B, H, KV, nsplit, window, chunk, sinks, scale * LOG2E};
   if (D == 128) {
     hipLaunchKernelGGL(decode_partial_kernel<128>, dim3(B * KV, nsplit), dim3(256), 0, stream, a);
     hipLaunchKernelGGL(decode_combine_kernel<128>, dim3(B * H), dim3(128), 0, stream, a);

@@ -34,6 +34,7 @@ class ModelConfig:
     sliding_window: int = 0  # 0 = full causal
     tie_embeddings: bool = False
     name: str = ""
+    attention_sinks: int = 0  # with a sliding window: this many first tokens stay visible to every later one
     extra: dict = field(default_factory=dict)
 
     @property
@@ -85,6 +86,8 @@ class ModelConfig:
                "tie_word_embeddings": self.tie_embeddings, "torch_dtype": "bfloat16"}
         if self.sliding_window:
             cfg["sliding_window"] = self.sliding_window
+        if self.attention_sinks:
+            cfg["attention_sinks"] = self.attention_sinks
         if self.rope_scaling:
             cfg["rope_scaling"] = self.rope_scaling
         # transformers >= 5 reads RoPE only from "rope_parameters" (the top-level keys above serve 4.x)
@@ -116,7 +119,8 @@ class ModelConfig:
                    cfg.get("num_key_value_heads", cfg["num_attention_heads"]), cfg["intermediate_size"],
                    cfg.get("max_position_embeddings", 8192), theta, scaling,
                    cfg.get("rms_norm_eps", 1e-5), cfg.get("sliding_window") or 0,
-                   cfg.get("tie_word_embeddings", False), name=name or mt)
+                   cfg.get("tie_word_embeddings", False), name=name or mt,
+                   attention_sinks=cfg.get("attention_sinks") or 0)
 
 
 _L31 = {"rope_type": "llama3", "factor": 8.0, "low_freq_factor": 1.0, "high_freq_factor": 4.0,
@@ -149,8 +153,19 @@ PRESETS: dict[str, ModelConfig] = {
 }
 
 
-def get_config(name_or_path: str) -> ModelConfig:
+def get_config(name_or_path: str, sliding_window: int = -1, attention_sinks: int = -1) -> ModelConfig:
+    """A preset or an HF ``config.json``; ``sliding_window`` / ``attention_sinks`` >= 0 replace the model's own."""
     if name_or_path in PRESETS:
-        return dataclasses.replace(PRESETS[name_or_path])
-    with open(name_or_path) as f:
-        return ModelConfig.from_hf_config(json.load(f))
+        cfg = dataclasses.replace(PRESETS[name_or_path])
+    else:
+        with open(name_or_path) as f:
+            cfg = ModelConfig.from_hf_config(json.load(f))
+    if sliding_window >= 0:
+        cfg.sliding_window = sliding_window
+    if attention_sinks >= 0:
+        cfg.attention_sinks = attention_sinks
+    if cfg.family != "llama" and (cfg.sliding_window or cfg.attention_sinks):
+        raise ValueError(f"{cfg.name or cfg.family}: a sliding window and sinks are for the Llama / Mistral trunk")
+    if cfg.attention_sinks and not cfg.sliding_window:
+        raise ValueError("attention_sinks needs a sliding window (without one every token is visible)")
+    return cfg

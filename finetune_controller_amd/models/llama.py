@@ -1,4 +1,5 @@
-"""Llama-3 / Mistral decoder (one trunk; Mistral = sliding-window attention + its own vocab/RoPE).
+"""Llama-3 / Mistral decoder (one trunk; Mistral = sliding-window attention (optionally with
+sinks: the first keys stay visible) + its own vocab/RoPE).
 
 MI355X-first layout decisions (not a port of any reference module -- the reference has no model
 code):
@@ -160,8 +161,7 @@ class LlamaLayer(nn.Module):
                                         handoff=rgrad)
         if kv is not None and kv[0].decoding:  # generation: one new token per sequence vs its cache
             cache, li = kv
-            a = ops.decode_attention(qkv, cache.k[li], cache.v[li], cache.lens_next, cache.attend_len(),
-                                     cfg.n_heads, cfg.n_kv_heads, cfg.head_dim, window=cfg.sliding_window)
+            a = cache.attend(li, qkv, cfg.n_heads, cfg.sliding_window, cfg.attention_sinks)
         else:
             if kv is not None:  # prefill: keep this prompt's K/V rows
                 kv[0].store(kv[1], qkv, cfg.n_heads, S)
@@ -169,11 +169,12 @@ class LlamaLayer(nn.Module):
             if sp is not None and kv is None:  # Ulysses: heads <-> tokens all-to-all around full-sequence attention
                 from ..parallel.sequence import sp_attention
 
-                a = sp_attention(qkv, B, S, cfg.n_heads, cfg.n_kv_heads, cfg.head_dim, cfg.sliding_window, sp)
+                a = sp_attention(qkv, B, S, cfg.n_heads, cfg.n_kv_heads, cfg.head_dim, cfg.sliding_window, sp,
+                                 cfg.attention_sinks)
             else:
                 a = ops.attention_packed(qkv, B, S, cfg.n_heads, cfg.n_kv_heads, cfg.head_dim, True,
                                          cfg.sliding_window, out_pad=p_o, grad_pad=p_qkv, docs=docs,
-                                         rope_grad=rgrad)
+                                         rope_grad=rgrad, sinks=cfg.attention_sinks)
         o = self.proj("o", a)
         h, x = ops.add_rms_norm(h, o, self.mlp_norm, cfg.norm_eps, pad=p_gu, grad_pad=p_o)
         mlp = self.mlp_projs(p_gu, p_down)

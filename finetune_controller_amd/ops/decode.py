@@ -29,7 +29,7 @@ def visible_keys(n: torch.Tensor, L: int, window: int = 0, sinks: int = 0) -> to
 
 
 def decode_attention_reference(q, k_cache, v_cache, lens, H: int, KV: int, D: int, scale: float,
-                               window: int = 0) -> torch.Tensor:
+                               window: int = 0, sinks: int = 0) -> torch.Tensor:
     """q [B, >=H*D]; caches [B, Lmax, KV*D]; lens [B] valid keys -> [B, H*D] (fp32 math)."""
     B, L = k_cache.shape[0], k_cache.shape[1]
     G = H // KV
@@ -37,11 +37,7 @@ def decode_attention_reference(q, k_cache, v_cache, lens, H: int, KV: int, D: in
     k = k_cache.float().view(B, L, KV, D)
     v = v_cache.float().view(B, L, KV, D)
     s = torch.einsum("bkgd,blkd->bkgl", qf, k) * scale
-    t = torch.arange(L, device=q.device)
-    n = lens.to(q.device).long().view(B, 1)
-    ok = t[None, :] < n
-    if window and window > 0:
-        ok &= t[None, :] >= (n - window)
+    ok = visible_keys(lens.to(q.device), L, window, sinks)
     s = s.masked_fill(~ok[:, None, None, :], float("-inf"))
     p = s.softmax(-1)
     o = torch.einsum("bkgl,blkd->bkgd", p, v)
@@ -49,18 +45,22 @@ def decode_attention_reference(q, k_cache, v_cache, lens, H: int, KV: int, D: in
 
 
 def decode_attention(qkv, k_cache, v_cache, lens, max_len: int, H: int, KV: int, D: int, scale: float | None = None,
-                     window: int = 0) -> torch.Tensor:
+                     window: int = 0, sinks: int = 0) -> torch.Tensor:
     """One query token per sequence against its cache.  ``qkv`` [B, (H+2KV)*D]: the current token's
     packed projection, whose K / V rows are appended at position ``lens - 1`` (the HIP kernel does it
-    while attending); ``max_len`` (host int) bounds ``lens``."""
+    while attending); ``max_len`` (host int) bounds ``lens``.  ``window`` > 0: the last
+    ``window`` keys and the first ``sinks`` are seen."""
+    if sinks < 0:
+        raise ValueError(f"decode_attention: sinks must not be negative, got {sinks}")
     scale = scale if scale is not None else 1.0 / math.sqrt(D)
     if use_hip(qkv) and qkv.dtype == torch.bfloat16 and D in (64, 128) and H // KV <= 8:
-        return ext().decode_attention(qkv, k_cache, v_cache, lens, H, KV, D, int(max_len), scale, int(window or 0))
+        return ext().decode_attention(qkv, k_cache, v_cache, lens, H, KV, D, int(max_len), scale, int(window or 0),
+                                      int(sinks))
     B, kv = qkv.shape[0], KV * D
     rows, pos = torch.arange(B, device=qkv.device), lens.long() - 1
     k_cache.index_put_((rows, pos), qkv[:, H * D:H * D + kv])
     v_cache.index_put_((rows, pos), qkv[:, H * D + kv:H * D + 2 * kv])
-    return decode_attention_reference(qkv, k_cache, v_cache, lens, H, KV, D, scale, window)
+    return decode_attention_reference(qkv, k_cache, v_cache, lens, H, KV, D, scale, window, sinks)
 
 
 class KVCache:
@@ -68,8 +68,11 @@ class KVCache:
     so no step needs a device read) advance together."""
 
     def __init__(self, n_layers: int, B: int, max_len: int, KV: int, D: int, device, dtype=torch.bfloat16):
+        self._init_lens(B, max_len, KV, D, device)
         self.k = torch.zeros(n_layers, B, max_len, KV * D, device=device, dtype=dtype)
         self.v = torch.zeros_like(self.k)
+
+    def _init_lens(self, B: int, max_len: int, KV: int, D: int, device):
         self.B, self.max_len, self.KV, self.D = B, max_len, KV, D
         self.lens = torch.zeros(B, dtype=torch.int32, device=device)
         self.host_lens = [0] * B
@@ -83,6 +86,11 @@ class KVCache:
         kv = self.KV * self.D
         self.k[layer, self.row, :S].copy_(qkv[:, H * self.D:H * self.D + kv].view(S, kv))
         self.v[layer, self.row, :S].copy_(qkv[:, H * self.D + kv:H * self.D + 2 * kv].view(S, kv))
+
+    def attend(self, layer: int, qkv: torch.Tensor, H: int, window: int = 0, sinks: int = 0) -> torch.Tensor:
+        """Decode step of one layer: append the current tokens' K / V rows and attend -> [B, H*D]."""
+        return decode_attention(qkv, self.k[layer], self.v[layer], self.lens_next, self.attend_len(), H, self.KV, self.D,
+                                window=window, sinks=sinks)
 
     def begin_decode(self):
         """Positions of the tokens about to be appended (= current lengths); ``lens_next`` (their

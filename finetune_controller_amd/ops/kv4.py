@@ -26,6 +26,7 @@ import math
 import torch
 
 from ._backend import ext, use_hip
+from .decode import KVCache, visible_keys
 
 KV4_TILE = 32   # tokens per record
 KV4_GROUP = 32  # values per scale
@@ -199,8 +200,6 @@ def decode_attention_kv4_reference(q, data, lens, H: int, KV: int, D: int, scale
                                    sinks: int = 0) -> torch.Tensor:
     """q [B, >=H*D] against the first ``lens`` tokens of the cache -> [B, H*D] (fp32 math).  A sequence with
     no visible token gives a zero row."""
-    from .decode import visible_keys
-
     B, cap = data.shape[0], data.shape[2] * KV4_TILE
     qf = q[:, :H * D].float().reshape(B, KV, H // KV, D)
     n = lens.long().clamp(max=cap)
@@ -240,3 +239,22 @@ def decode_attention_kv4(qkv: torch.Tensor, data: torch.Tensor, lens: torch.Tens
     new = qkv[:, H * D:(H + 2 * KV) * D].unflatten(1, (2, KV * D))
     kv4_store(data, new[:, None, 0], new[:, None, 1], torch.where(lens <= max_len, lens - 1, lens - lens - 1))
     return decode_attention_kv4_reference(qkv, data, lens.clamp(max=max_len), H, KV, D, scale, window, sinks)
+
+
+class KV4Cache(KVCache):
+    """``KVCache`` with its rows held in 4 bits: ``data`` [n_layers, B, KV, tiles, record].  Prefill attends over the
+    prompt's own rows and stores them quantised; decode steps attend over the quantised cache."""
+
+    def __init__(self, n_layers: int, B: int, max_len: int, KV: int, D: int, device):
+        self._init_lens(B, max_len, KV, D, device)
+        self.data = kv4_alloc(B, max_len, KV, D, device, layers=n_layers)
+        self._zero = torch.zeros(1, dtype=torch.int32, device=device)
+
+    def store(self, layer: int, qkv: torch.Tensor, H: int, S: int):
+        k0, v0 = H * self.D, (H + self.KV) * self.D
+        rows = qkv[None, :S]
+        kv4_store(self.data[layer, self.row:self.row + 1], rows[..., k0:v0], rows[..., v0:v0 + self.KV * self.D], self._zero)
+
+    def attend(self, layer: int, qkv: torch.Tensor, H: int, window: int = 0, sinks: int = 0) -> torch.Tensor:
+        return decode_attention_kv4(qkv, self.data[layer], self.lens_next, self.attend_len(), H, self.KV, self.D,
+                                    window=window, sinks=sinks)

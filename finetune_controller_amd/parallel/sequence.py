@@ -147,7 +147,7 @@ class _OutToTokens(torch.autograd.Function):
 
 
 def sp_attention(qkv: torch.Tensor, B: int, S_local: int, H: int, KV: int, D: int, window: int,
-                 sp: SeqGroup) -> torch.Tensor:
+                 sp: SeqGroup, sinks: int = 0) -> torch.Tensor:
     """Causal GQA attention over the full sequence of a sequence-parallel group; ``qkv`` holds this
     rank's ``S_local`` tokens of each of the B sequences (RoPE applied with global positions).  Returns
     this rank's tokens' attention output [B*S_local, H*D]."""
@@ -157,7 +157,7 @@ def sp_attention(qkv: torch.Tensor, B: int, S_local: int, H: int, KV: int, D: in
     if H % P or KV % P:
         raise ValueError(f"sequence parallel degree {P} must divide the query ({H}) and kv ({KV}) head counts")
     full = _QKVToHeads.apply(qkv, B, S_local, H, KV, D, sp)
-    a = attention_packed(full, B, P * S_local, H // P, KV // P, D, True, window)
+    a = attention_packed(full, B, P * S_local, H // P, KV // P, D, True, window, sinks=sinks)
     return _OutToTokens.apply(a, B, S_local, H, D, sp)
 
 

@@ -67,6 +67,10 @@ def build_parser() -> argparse.ArgumentParser:
                     help="EOS-separated documents in a window attend only within themselves (positions restart)")
     ap.add_argument("--completion-only", action="store_true",
                     help="prompt/completion records: no loss on prompt tokens")
+    ap.add_argument("--sliding-window", type=int, default=-1,
+                    help="attention window of the Llama / Mistral trunk (-1: the model's, 0: full causal)")
+    ap.add_argument("--attention-sinks", type=int, default=-1,
+                    help="first tokens that stay visible beside the sliding window (-1: the model's)")
     ap.add_argument("--eos-id", type=int, default=-1, help="document separator (-1: the dataset tokenizer's EOS)")
     ap.add_argument("--eval-every", type=int, default=0, help="held-out loss every N steps (0: off)")
     ap.add_argument("--eval-batches", type=int, default=4, help="micro-batches per rank per evaluation")
@@ -103,7 +107,8 @@ def config_from_args(a) -> TrainConfig:
                        dtype=a.dtype, device=a.device, timers=a.timers, profile_steps=a.profile_steps,
                        eval_every=a.eval_every, eval_batches=a.eval_batches, eval_holdout=a.eval_holdout,
                        pack_documents=a.pack_documents, eos_id=a.eos_id,
-                       completion_only=a.completion_only, graph=a.graph,
+                       completion_only=a.completion_only, graph=a.graph, sliding_window=a.sliding_window,
+                       attention_sinks=a.attention_sinks,
                        step_timeout_s=a.step_timeout)
 
 

@@ -99,6 +99,8 @@ class TrainConfig:
     pack_documents: bool = False  # EOS-separated documents in a window attend only within themselves
     eos_id: int = -1  # -1: the dataset tokenizer's EOS (tokenizer.json, or the byte-level fallback's 2)
     completion_only: bool = False  # prompt/completion records: loss on the completion tokens only
+    sliding_window: int = -1  # attention window of the Llama / Mistral trunk (-1: the model's, 0: full causal)
+    attention_sinks: int = -1  # first tokens that stay visible beside the window (-1: the model's)
     synthetic_doc_len: int = 0  # synthetic data: EOS every that many tokens (packed-document benchmarks)
     step_timeout_s: float = 0.0  # >0: exit 124 when no step / eval / save finishes for that long (FTC_STEP_TIMEOUT_S)
     # device events around the gradient-reduction wait of every step: the comm time backward did not
@@ -133,7 +135,9 @@ class Trainer:
         else:
             self.dtype = {"bf16": torch.bfloat16, "fp32": torch.float32, "bfloat16": torch.bfloat16,
                           "float32": torch.float32}[tc.dtype]
-        self.cfg = get_config(tc.model)
+        self.cfg = get_config(tc.model, tc.sliding_window, tc.attention_sinks)
+        if self.cfg.attention_sinks and tc.pack_documents:
+            raise ValueError("attention_sinks and pack_documents do not go together (one document per sequence only)")
         if tc.seq_len > self.cfg.max_seq_len:
             self.cfg.max_seq_len = tc.seq_len
         self.lora = tc.lora_config()
