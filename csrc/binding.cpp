@@ -546,7 +546,7 @@ void flash_bwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, co
 
 // ---------------- flash attention with a window and sinks (csrc/kernels/flash_sink.hip) ----------------
 // q, k, v are head-column views of one packed [B*S, (H+2KV)*D] projection (16-byte aligned rows), any S.
-// grad: the output's low bits (uint8, a [0, H*D] tensor otherwise) are kept for the backward.
+// grad: the output's low bits (uint8) and the LSE are kept for the backward (empty tensors otherwise).
 inline void need_packed(const at::Tensor& qkv, int64_t B, int64_t S, int64_t W, const char* name) {
   need(qkv, at::kBFloat16, name);
   TORCH_CHECK(qkv.dim() == 2 && qkv.size(0) == B * S && qkv.size(1) >= W && qkv.stride(1) == 1 &&
@@ -568,7 +568,7 @@ std::vector<at::Tensor> sink_fwd(const at::Tensor& qkv, int64_t B, int64_t S, in
   c10::DeviceGuard guard(qkv.device());
   auto obuf = at::empty({B * S, H * D + pad}, qkv.options());
   auto o = pad ? obuf.narrow(1, 0, H * D) : obuf;
-  auto lse = at::empty({B, H, S}, qkv.options().dtype(at::kFloat));
+  auto lse = at::empty({grad ? B : 0, H, S}, qkv.options().dtype(at::kFloat));
   auto olow = at::empty({grad ? B * S : 0, H * D}, qkv.options().dtype(at::kByte));
   const auto* p = static_cast<const uint16_t*>(qkv.data_ptr());
   check(ftc_sink_fwd(p, p + H * D, p + (H + KV) * D, o.data_ptr(), grad ? olow.data_ptr() : nullptr, lse.data_ptr<float>(), (int)B, (int)S, (int)H, (int)KV,

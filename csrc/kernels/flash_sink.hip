@@ -67,9 +67,9 @@ DEV_INLINE float with_low_byte(uint32_t hi, uint32_t byte) {  // hi: the bf16 in
   return __uint_as_float(hi + ((uint32_t)((int)(byte << 24) >> 24) << 8));
 }
 
-// GRAD: the output is for a backward pass as well: its low bits are kept, and O is normalised by the sum of the weights
-// as they were rounded for the PV product (one more MFMA column of ones), so that the rounding of a row's largest
-// weights cancels; the LSE keeps the 32-bit sum.
+// O is normalised by the sum of the weights as they were rounded for the PV product, so that the rounding of a row's
+// largest weights cancels (and 16 two-element dot products replace 32 adds a tile).  GRAD: a backward pass follows --
+// the output's low bits are kept, and the LSE of the unrounded weights.
 template <int D, bool GRAD>
 __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void sink_fwd_kernel(FwdArgs a) {
   constexpr int BQ = 32 * WAVES;
@@ -147,8 +147,7 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void sink_fwd_kernel(FwdArgs
     for (int i = 0; i < 16; ++i) o[t][i] = 0.f;
   float m = -INFINITY, l = 0.f;
   const float c = a.scale_log2;
-  f32x16 lr_ = {};  // GRAD: sum of the rounded weights (every element)
-  const bf16x8 ones = as_bf8(make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u));
+  float lw = 0.f;  // sum of the weights as rounded for the PV product
 
   __builtin_amdgcn_s_waitcnt(0x0F70);  // Q fragments (plain loads) retired before any DMA: vmcnt(0)
   dma(tile_key(0), K0, V0);
@@ -241,10 +240,7 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void sink_fwd_kernel(FwdArgs
       for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[dt][i] *= alpha;
-      if constexpr (GRAD) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) lr_[i] *= alpha;
-      }
+      lw *= alpha;
     }
     const float mref = (m == -INFINITY) ? 0.f : m;
     float rs = 0.f;
@@ -254,18 +250,22 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void sink_fwd_kernel(FwdArgs
       for (int i = 0; i < 16; ++i) {
         const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][i], c, -mref));
         s[kt][i] = p;
-        rs += p;
+        if constexpr (GRAD) rs += p;
       }
-    l += rs;
+    if constexpr (GRAD) l += rs;
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) pf[ks] = pack8_bf(s[ks >> 1], 8 * (ks & 1));
+    for (int ks = 0; ks < 4; ++ks) {
+      uint32_t w[4];  // summed from the words: taken back out of the operand vector, hipcc 7.2 sums its first word 4 times
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        w[i] = pack_bf2(s[ks >> 1][8 * (ks & 1) + 2 * i], s[ks >> 1][8 * (ks & 1) + 2 * i + 1]);
+        lw = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w[i]), __builtin_bit_cast(bf16x2, 0x3f803f80u), lw, false);
+      }
+      pf[ks] = as_bf8(make_uint4(w[0], w[1], w[2], w[3]));
+    }
   };
   // ---- phase B2: O^T += V^T P^T, 4 k-steps of 16 keys
   auto phaseB2 = [&](const char* Vc) __attribute__((always_inline)) {
-    if constexpr (GRAD) {
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks) lr_ = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ones, pf[ks], lr_, 0, 0, 0);
-    }
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
       s16x4 vt[8];  // all 8 transposed reads of this 32-wide d tile in flight before the MFMA chain
@@ -302,8 +302,8 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void sink_fwd_kernel(FwdArgs
   }
 
   // ---- epilogue: normalise, store O (bf16) and LSE (natural log)
-  const float ltot = l + __shfl_xor(l, 32, 64);
-  const float lnorm = GRAD ? lr_[0] : ltot, inv = lnorm > 0.f ? 1.0f / lnorm : 0.f;
+  lw += __shfl_xor(lw, 32, 64);
+  const float inv = lw > 0.f ? 1.0f / lw : 0.f;
   uint16_t* op = a.o + ((long long)b * S + (qvalid ? qrow : 0)) * a.o_rs + (long long)hq * D;
   if constexpr (GRAD) {
     // the 4 bytes of each g4 are a dword; two swaps give lane half hh the 16 bytes of d [16 hh, 16 hh + 16)
@@ -356,8 +356,9 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void sink_fwd_kernel(FwdArgs
         *reinterpret_cast<uint2*>(op + d) = w;
       }
   }
-  if (qvalid) {
-    if (hh == 0) {
+  if constexpr (GRAD) {
+    const float ltot = l + __shfl_xor(l, 32, 64);
+    if (qvalid && hh == 0) {
       const float lse2 = (m == -INFINITY) ? -INFINITY : m + __log2f(ltot);
       a.lse[((long long)b * a.H + hq) * S + qrow] = lse2 * LN2;
     }
@@ -795,19 +796,31 @@ __global__ __launch_bounds__(64 * FAR_WAVES, 1) void sink_far_kernel(BwdArgs a) 
   const int sl0 = (key0 + a.window) / 32, nsl = (S + 31) / 32 - sl0;  // slices that hold far queries of these keys
   const int total = nsl > 0 ? nsl * G : 0, per = (total + a.nfar - 1) / a.nfar;
   const int t1 = min(total, (part + 1) * per);
-  for (int t = part * per + wave; t < t1; t += FAR_WAVES) {
-    const int qt = (sl0 + t / G) * 32, hq = kvh * G + t % G;
-    const int row = min(qt + lr, S - 1);
+  uint4 qa[DSTEPS], da[DSTEPS], qn[DSTEPS], dn[DSTEPS];
+  float cst = 0.f, cn = 0.f;
+  auto fetch = [&](int t) __attribute__((always_inline)) {  // slice t's rows, into the next registers
+    const int qt = (sl0 + t / G) * 32, hq = kvh * G + t % G, row = min(qt + lr, S - 1);
     const uint16_t* qp = a.q + ((long long)b * S + row) * a.q_rs + (long long)hq * D + 8 * hh;
-    const uint16_t* dp_ = a.dout + ((long long)b * S + row) * a.do_rs + (long long)hq * D + 8 * hh;
-    uint4 qa[DSTEPS], da[DSTEPS];
+    const uint16_t* dp = a.dout + ((long long)b * S + row) * a.do_rs + (long long)hq * D + 8 * hh;
 #pragma unroll
     for (int st = 0; st < DSTEPS; ++st) {
-      qa[st] = *reinterpret_cast<const uint4*>(qp + 16 * st);
-      da[st] = *reinterpret_cast<const uint4*>(dp_ + 16 * st);
+      qn[st] = *reinterpret_cast<const uint4*>(qp + 16 * st);
+      dn[st] = *reinterpret_cast<const uint4*>(dp + 16 * st);
     }
-    const long long cidx = ((long long)b * a.H + hq) * S + row;
-    const float cst = a.delta[cidx + (hh ? 0 : (long long)a.B * a.H * S)];  // lanes 0..31 -lse/scale, 32..63 -delta
+    // lanes 0..31 -lse/scale, 32..63 -delta
+    cn = a.delta[((long long)b * a.H + hq) * S + row + (hh ? 0 : (long long)a.B * a.H * S)];
+  };
+  int t = part * per + wave;
+  if (t < t1) fetch(t);
+  for (; t < t1; t += FAR_WAVES) {
+    const int qt = (sl0 + t / G) * 32;
+#pragma unroll
+    for (int st = 0; st < DSTEPS; ++st) {
+      qa[st] = qn[st];
+      da[st] = dn[st];
+    }
+    cst = cn;
+    fetch(min(t + FAR_WAVES, t1 - 1));
 #pragma unroll
     for (int st = 0; st < DSTEPS; ++st) {
       *reinterpret_cast<uint4*>(Qs + lds_off<D>(lr, 2 * st + hh)) = qa[st];
