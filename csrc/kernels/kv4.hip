@@ -51,7 +51,7 @@ __global__ __launch_bounds__(256) void kv4_store_kernel(StoreArgs a) {
   const long long tile = p0 / KV4_TILE + sp;
   if (tile >= a.tiles) return;
   const long long row0 = tile * KV4_TILE - start;  // row index of the record's token 0
-  if (row0 >= n || row0 + KV4_TILE <= 0) return;
+  if (n < 1 || row0 >= n || row0 + KV4_TILE <= 0) return;
   const bool whole = row0 >= 0 && row0 + KV4_TILE <= n;
   uint8_t* rec = a.data + (((long long)b * a.KV + kvh) * a.tiles + tile) * L::REC;
   const uint16_t* kp = a.k + b * a.k_bs + (long long)kvh * D;

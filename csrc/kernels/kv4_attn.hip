@@ -418,14 +418,17 @@ Plan kv4_plan(int B, int H, int KV, int D, int max_len, int window, int sinks) {
   // split from 1 to 128: it picks the quickest or one within 4 % (one 32768-token sequence, 8 items: 32 parts
   // 15.0 us, 24 parts 16.4, unsplit 192; 16 sequences at a 4096 window: 2 parts 18.9, 1 part 30.9; 32 x 4096
   // tokens: unsplit 25.3, 2 parts 30.0).
-  float best = 3e38f;
-  p.nsplit = 1;
-  const long long most = vis / p.nw < 1 ? 1 : (vis + p.nw - 1) / p.nw;
-  for (long long n = 1; n <= most && n <= 256; ++n) {
+  const long long most = (vis + p.nw - 1) / p.nw;
+  auto model = [&](long long n) {
     const long long rounds = (items * n + 255) / 256, per = ((vis + n - 1) / n + p.nw - 1) / p.nw;
-    const float us = rounds * (per * 1.8f + 2.5f) + (n > 1 ? 3.f : 0.f);
-    if (us < best) {
-      best = us;
+    return rounds * (per * 1.8f + 2.5f) + (n > 1 ? 3.f : 0.f);
+  };
+  p.nsplit = 1;
+  float best = model(1);
+  for (int r = 1; r <= 8; ++r) {  // the most parts that r rounds hold
+    const long long full = 256LL * r / items, n = full < most ? full : most;
+    if (n > 1 && n <= 256 && model(n) < best) {
+      best = model(n);
       p.nsplit = (int)n;
     }
   }

@@ -320,6 +320,13 @@ class _FlashPaddedTail(torch.autograd.Function):
         return dqkv, None, None, None, None, None, None, None, None, None, None, None
 
 
+def _rows16(t: torch.Tensor) -> torch.Tensor:
+    """``t`` itself if its rows can be read 16 bytes at a time, else a copy."""
+    if t.stride(1) == 1 and t.stride(0) >= t.shape[1] and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
 class _FlashSinks(torch.autograd.Function):
     """Window + sinks on ``csrc/kernels/flash_sink.hip``: any S; a head_dim the kernels are not built for runs on
     zero-padded heads (exact: see _FlashPaddedTail)."""
@@ -330,11 +337,7 @@ class _FlashSinks(torch.autograd.Function):
         Dp = kernel_head_dim(D)
         ctx.rope_grad = None
         if Dp == D:
-            x = qkv
-            if x.stride(1) != 1 or x.stride(0) % 8 or x.data_ptr() % 16:
-                x = x.contiguous()
-                if x.data_ptr() % 16:
-                    x = x.clone()
+            x = _rows16(qkv)
             o, olow, lse = ext().sink_fwd(x, B, S, H, KV, D, scale, window, sinks, out_pad, grad)
             out = o
             if rope_grad is not None and ROPE_BWD_FUSE and D == 128 and rope_grad.cos.shape[-1] == 64 and (
@@ -359,10 +362,7 @@ class _FlashSinks(torch.autograd.Function):
         nh = H + 2 * KV
         _gate_dw()
         if Dp == D:
-            if do.stride(1) != 1 or do.stride(0) % 8 or do.data_ptr() % 16:
-                do = do.contiguous()
-                if do.data_ptr() % 16:
-                    do = do.clone()
+            do = _rows16(do)
             extra = W - nh * D  # qkv was wider than its heads: those columns get no gradient
             g = ext().sink_bwd(x, ctx.o, olow, do, lse, B, S, H, KV, D, scale, window, sinks, grad_pad if not extra else 0,
                                rg.cos if rg is not None else None, rg.sin if rg is not None else None,

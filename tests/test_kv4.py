@@ -253,6 +253,10 @@ def test_store_kernel_writes_the_reference_bytes(D, KV, n, start):
         assert _same_held(got.cpu(), want, D)
         if n < 33:
             assert torch.equal(got.cpu(), want)
+    none, got = torch.zeros(B, dtype=torch.int32), old.cuda()  # no rows of a padded batch, or fewer than none
+    for cnt in (none, none - 7):
+        ops.kv4_store(got, g[..., :KV * D], g[..., KV * D:2 * KV * D], st.cuda(), cnt.cuda())
+    assert torch.equal(got.cpu(), old)
     off = g.flatten()[1:1 + B * n * KV * D].view(B, n, KV * D)  # rows that start off a 16-byte boundary
     want, got = old.clone(), old.cuda()
     ops.kv4_store(want, off.cpu(), off.cpu(), st)
@@ -310,6 +314,29 @@ def test_decode_kernel_long(D, H, KV):
     for window, sinks in ((0, 0), (4096, 4), (100, 33)):
         got = ops.decode_attention_kv4(qkv.cuda(), data, ln, 9000, H, KV, D, window=window, sinks=sinks)
         _check(got, *_expected(qkv, k, v, lens, H, KV, D, D ** -0.5, window, sinks))
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("max_len", [64, 120])
+def test_lengths_outside_the_bound(dev, max_len):
+    """Zero and negative lengths give zero rows; longer than max_len: its first max_len tokens, nothing written."""
+    B, H, KV, D, cap = 5, 4, 2, 64, 128
+    lens = (0, -3, max_len, max_len + 1, 2 ** 31 - 1)
+    qkv, k, v = _decode_case(B, H, KV, D, lens, cap, seed=21)
+    data = ops.kv4_alloc(B, cap, KV, D, device=dev)
+    ops.kv4_store(data, k.to(dev), v.to(dev), torch.zeros(B, dtype=torch.int32, device=dev))
+    before = data.clone()
+    ln = torch.tensor(lens, dtype=torch.int32, device=dev)
+    got = ops.decode_attention_kv4(qkv.to(dev), data, ln, max_len, H, KV, D).cpu()
+    assert (got[:2] == 0).all()
+    ops.kv4_store(before[2:3], qkv[2:3, None, H * D:(H + KV) * D].to(dev), qkv[2:3, None, (H + KV) * D:].to(dev), ln[2:3] - 1)
+    assert torch.equal(before, data)
+    want, pv = _expected(qkv[2:3], k[2:3], v[2:3], (max_len,), H, KV, D, D ** -0.5, 0, 0)
+    _check(got[2:3], want, pv)
+    for b in (3, 4):
+        K, V = (_codes_of(t[b].unflatten(-1, (KV, D))).flatten(-2) for t in (k, v))
+        o, p = _attend64(qkv[b], K, V, torch.arange(cap) < max_len, H, KV, D, D ** -0.5)
+        _check(got[b], o, p)
 
 
 @pytest.mark.gpu

@@ -164,6 +164,23 @@ def test_views_and_padded_buffers(S, window):
 
 
 @pytest.mark.gpu
+def test_expanded_and_single_row_gradients():
+    """Output gradients as autograd makes them: one row expanded over all, a single row with an odd row stride."""
+    H, KV, D, window, sinks = 2, 1, 64, 7, 2
+    for S in (40, 1):
+        qkv, do = _inputs(1, S, H, KV, D, seed=8)
+        do = do[:1].expand(S, -1)
+        _, _, wg, tg = _definition(qkv, do.contiguous(), 1, S, H, KV, D, window, sinks, D ** -0.5)
+        odd = torch.empty(S, H * D + 5, dtype=BF, device="cuda")[:, :H * D]
+        odd.copy_(do.cuda())
+        for g_out in (do[:1].cuda().expand(S, -1), odd):
+            x = qkv.cuda().requires_grad_()
+            o = ops.attention_packed(x, 1, S, H, KV, D, window=window, sinks=sinks)
+            (g,) = torch.autograd.grad(o, x, g_out)
+            _close(g, wg, tg)
+
+
+@pytest.mark.gpu
 def test_rope_handoff():
     """The backward takes RoPE's inverse rotation into its epilogues (rows past a tile, positions given)."""
     B, S, H, KV, D, window, sinks = 2, 290, 2, 1, 128, 64, 4
