@@ -5,8 +5,9 @@
 //   K  chunk of lane (r, q): token t(half, r) = 8 (r >> 2) + 4 half + (r & 3); word j holds d = 32 j + 8 q
 //      + 0..7, even d in the low 16 bits (nibbles d/2), odd d in the high 16 bits.
 //      D = 128: chunk half = 4 words (j = 0..3), two chunks 1 KiB apart; D = 64: one chunk, words [half][j].
-//   V  chunk of lane (r, q): tokens 8 q + 0..7, d = (D/16) r + 4 quad + 0..3; word p holds tokens 2p (low 16
-//      bits) and 2p + 1 (high), nibble i = d0 + i.  D = 128: two chunks (quad) 1 KiB apart; D = 64: one.
+//   V  chunk c of lane (r, q): tokens 8 q + 0..7, d = 64 c + 4 r + 0..3; word p holds tokens 2p (low 16 bits) and
+//      2p + 1 (high), nibble i = d0 + i.  The 16 rows r of an MFMA so lie in two value groups, 2 c + (r >> 3).
+//      Chunks are 1 KiB apart.
 //   scales (bf16): chunk (q, g) of 8 tokens 8 q + 0..7 of value group g = d / 32.
 // (x >> 4 i) & 0x000f000f of a word is therefore a pair of adjacent MFMA k elements: two d of one token (K), two
 // tokens of one d (V) -- unpacking costs one shift and one and-or a pair and no cross-lane traffic.
@@ -22,7 +23,6 @@ constexpr int KV4_TILE = 32, KV4_GROUP = 32;
 template <int D>
 struct Kv4 {
   static constexpr int NG = D / 32;                 // value groups (scales) per row
-  static constexpr int NJ = D / 16;                 // d per V lane row
   static constexpr int CH = D / 64;                 // 16-byte chunks per lane and matrix
   static constexpr int CODES = KV4_TILE * D / 2;    // bytes
   static constexpr int SCALES = KV4_TILE * NG * 2;  // bytes
@@ -36,9 +36,8 @@ struct Kv4 {
     *soff = KS + ((t >> 3) * NG + j) * 16 + (t & 7) * 2;
   }
   DEV_INLINE static void v_at(int t, int d, int* off, int* shift, int* soff) {
-    const int r = d / NJ, jj = d % NJ;
-    *off = VC + (jj >> 2) * 1024 + (t >> 3) * 256 + r * 16 + (t & 7) * 2 + ((jj >> 1) & 1);
-    *shift = 4 * (jj & 1);
+    *off = VC + (d >> 6) * 1024 + (t >> 3) * 256 + ((d & 63) >> 2) * 16 + (t & 7) * 2 + ((d >> 1) & 1);
+    *shift = 4 * (d & 1);
     *soff = VS + ((t >> 3) * NG + (d >> 5)) * 16 + (t & 7) * 2;
   }
 };

@@ -3,7 +3,7 @@
 //
 // One wave = one record (32 tokens of one kv head).  A lane quantises exactly the 16-byte chunks that the
 // layout gives it: for K its token's 8-value runs of every group (the group maximum is shared by the 4 lanes of
-// that token), for V 8 tokens x 8 (4) values (shared by the lanes of the group), so nothing goes through LDS
+// that token), for V 8 tokens x 4 values of each 64 (shared by the lanes of the group), so nothing goes through LDS
 // and whole records are written as linear 16-byte stores.  Records that are only partly covered by the call
 // (its first and last, and every single-token append) store token by token; other tokens' bytes stay.
 // Bound: HBM -- 2 bytes read and 0.5625 written per value (and back).
@@ -68,16 +68,12 @@ __global__ __launch_bounds__(256) void kv4_store_kernel(StoreArgs a) {
 #pragma unroll
     for (int j = 0; j < L::NG; ++j) ku[half][j] = *reinterpret_cast<const uint4*>(p + 32 * j);
   }
-  uint4 vu[8];
+  uint2 vu[8][L::CH];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const uint16_t* p = vp + row_of(8 * q + i) * a.v_rs + L::NJ * r;
-    if constexpr (D == 128) {
-      vu[i] = *reinterpret_cast<const uint4*>(p);
-    } else {
-      const uint2 u = *reinterpret_cast<const uint2*>(p);
-      vu[i] = make_uint4(u.x, u.y, 0, 0);
-    }
+    const uint16_t* p = vp + row_of(8 * q + i) * a.v_rs + 4 * r;
+#pragma unroll
+    for (int c = 0; c < L::CH; ++c) vu[i][c] = *reinterpret_cast<const uint2*>(p + 64 * c);
   }
 
   // ---- K: this lane's token of each half, 8 values of every group
@@ -106,42 +102,41 @@ __global__ __launch_bounds__(256) void kv4_store_kernel(StoreArgs a) {
     }
   }
 
-  // ---- V: tokens 8 q + 0..7, NJ values from d = NJ r
-  uint32_t w[L::CH][4], sc[4];
+  // ---- V: tokens 8 q + 0..7, 4 values of each 64 (their group's maximum over the 8 lanes that share it)
 #pragma unroll
-  for (int p = 0; p < 4; ++p) {
-#pragma unroll
-    for (int c = 0; c < L::CH; ++c) w[c][p] = 0;
-    sc[p] = 0;
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    float f[8], rinv;
-    uint32_t key = keys8(vu[i]);  // (the zeros past 4 values at D = 64 raise no maximum)
-    unpack8(vu[i], f);
-    key = kv4_max2(key, kv4_dpp(key, 1));
-    key = kv4_max2(key, kv4_dpp(key, 2));
-    if constexpr (D == 64) key = kv4_max2(key, kv4_dpp(key, 3));
-    sc[i >> 1] |= kv4_scale(key_top(key), &rinv) << (16 * (i & 1));
-#pragma unroll
-    for (int c = 0; c < L::CH; ++c) w[c][i >> 1] |= kv4_pack_v(f + 4 * c, rinv) << (16 * (i & 1));
-  }
-  constexpr int LPG = 16 / L::NG;  // lanes r per group
-  if (whole) {
-#pragma unroll
-    for (int c = 0; c < L::CH; ++c)
-      *reinterpret_cast<uint4*>(rec + L::VC + c * 1024 + lane * 16) = make_uint4(w[c][0], w[c][1], w[c][2], w[c][3]);
-    if (r % LPG == 0)
-      *reinterpret_cast<uint4*>(rec + L::VS + (q * L::NG + r / LPG) * 16) = make_uint4(sc[0], sc[1], sc[2], sc[3]);
-  } else {
+  for (int c = 0; c < L::CH; ++c) {
+    uint32_t w[4], sc[4];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      if (!valid(8 * q + i)) continue;
+      const uint2 u = vu[i][c];
+      uint32_t key = kv4_max2(kv4_keys(u.x), kv4_keys(u.y));
+      key = kv4_max2(key, kv4_dpp(key, 1));
+      key = kv4_max2(key, kv4_dpp(key, 2));
+      key = kv4_max2(key, kv4_dpp(key, 3));
+      float rinv;
+      const uint32_t s = kv4_scale(key_top(key), &rinv);
+      const float f[4] = {bf_lo(u.x), bf_hi(u.x), bf_lo(u.y), bf_hi(u.y)};
+      const uint32_t n = kv4_pack_v(f, rinv);
+      if (i & 1) {
+        w[i >> 1] |= n << 16;
+        sc[i >> 1] |= s << 16;
+      } else {
+        w[i >> 1] = n;
+        sc[i >> 1] = s;
+      }
+    }
+    uint8_t* wp = rec + L::VC + c * 1024 + lane * 16;
+    uint8_t* sp = rec + L::VS + (q * L::NG + 2 * c + (r >> 3)) * 16;
+    if (whole) {
+      *reinterpret_cast<uint4*>(wp) = make_uint4(w[0], w[1], w[2], w[3]);
+      if (!(r & 7)) *reinterpret_cast<uint4*>(sp) = make_uint4(sc[0], sc[1], sc[2], sc[3]);
+    } else {
 #pragma unroll
-      for (int c = 0; c < L::CH; ++c)
-        *reinterpret_cast<uint16_t*>(rec + L::VC + c * 1024 + lane * 16 + 2 * i) = (uint16_t)(w[c][i >> 1] >> (16 * (i & 1)));
-      if (r % LPG == 0)
-        *reinterpret_cast<uint16_t*>(rec + L::VS + (q * L::NG + r / LPG) * 16 + 2 * i) = (uint16_t)(sc[i >> 1] >> (16 * (i & 1)));
+      for (int i = 0; i < 8; ++i) {
+        if (!valid(8 * q + i)) continue;
+        *reinterpret_cast<uint16_t*>(wp + 2 * i) = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+        if (!(r & 7)) *reinterpret_cast<uint16_t*>(sp + 2 * i) = (uint16_t)(sc[i >> 1] >> (16 * (i & 1)));
+      }
     }
   }
 }
@@ -206,11 +201,12 @@ __global__ __launch_bounds__(256) void kv4_load_kernel(LoadArgs a) {
     kw[i] = *reinterpret_cast<const uint32_t*>(rec + off);
     ks[i] = bf2f(*reinterpret_cast<const uint16_t*>(rec + so));
   }
-  constexpr int LPG = 16 / L::NG;
-  uint4 w[L::CH];
+  uint4 w[L::CH], sc[L::CH];
 #pragma unroll
-  for (int c = 0; c < L::CH; ++c) w[c] = *reinterpret_cast<const uint4*>(rec + L::VC + c * 1024 + lane * 16);
-  const uint4 sc = *reinterpret_cast<const uint4*>(rec + L::VS + (q * L::NG + r / LPG) * 16);
+  for (int c = 0; c < L::CH; ++c) {
+    w[c] = *reinterpret_cast<const uint4*>(rec + L::VC + c * 1024 + lane * 16);
+    sc[c] = *reinterpret_cast<const uint4*>(rec + L::VS + (q * L::NG + 2 * c + (r >> 3)) * 16);
+  }
 #pragma unroll
   for (int i = 0; i < 32 / RPI; ++i) {
     const int t = i * RPI + lane / CPR;
@@ -219,23 +215,20 @@ __global__ __launch_bounds__(256) void kv4_load_kernel(LoadArgs a) {
     for (int e = 0; e < 8; ++e) f[e] = ks[i] * ((float)(int)((kw[i] >> (16 * (e & 1) + 4 * (e >> 1))) & 15u) - 8.0f);
     if (valid(t)) *reinterpret_cast<uint4*>(kp + (row0 + t) * W + 8 * kc) = in ? pack8(f) : make_uint4(0, 0, 0, 0);
   }
-  float s[8];
-  unpack8(sc, s);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    if (!valid(8 * q + i)) continue;
-    float f[8];
+  for (int c = 0; c < L::CH; ++c) {
+    const uint32_t words[4] = {w[c].x, w[c].y, w[c].z, w[c].w};
+    float s[8];
+    unpack8(sc[c], s);
 #pragma unroll
-    for (int e = 0; e < L::NJ; ++e) {
-      const uint4& u = w[e >> 2];
-      const uint32_t x = (i >> 1) == 0 ? u.x : (i >> 1) == 1 ? u.y : (i >> 1) == 2 ? u.z : u.w;
-      f[e] = s[i] * ((float)(int)((x >> (16 * (i & 1) + 4 * (e & 3))) & 15u) - 8.0f);
+    for (int i = 0; i < 8; ++i) {
+      float f[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f[e] = s[i] * ((float)(int)((words[i >> 1] >> (16 * (i & 1) + 4 * e)) & 15u) - 8.0f);
+      if (valid(8 * q + i))
+        *reinterpret_cast<uint2*>(vp + (row0 + 8 * q + i) * W + 64 * c + 4 * r) =
+            in ? make_uint2(pack_bf2(f[0], f[1]), pack_bf2(f[2], f[3])) : make_uint2(0, 0);
     }
-    uint16_t* p = vp + (row0 + 8 * q + i) * W + L::NJ * r;
-    if constexpr (D == 128)
-      *reinterpret_cast<uint4*>(p) = in ? pack8(f) : make_uint4(0, 0, 0, 0);
-    else
-      *reinterpret_cast<uint2*>(p) = in ? make_uint2(pack_bf2(f[0], f[1]), pack_bf2(f[2], f[3])) : make_uint2(0, 0);
   }
 }
 

@@ -3,16 +3,19 @@
 // Work: one wave takes whole records (32 tokens of a kv head) for all query heads of the group, on the matrix
 // cores; the visible records of a sequence are split over workgroups and the partials joined by a second
 // kernel in a fixed order.
-//   columns of every MFMA = (query head h, value group g of 32): B = the head's q in group g's rows, zero
-//     elsewhere, so one chain of MFMAs over the head dimension gives the NG partial scores of a key apart and
-//     the group scales apply to the 32-bit results;
+//   columns of every MFMA = HPS query heads h x NGC = 16 / HPS value groups (of 32 d); NCH = NG / NGC chains take the
+//     groups NGC at a time.  B = the head's q in its column's group's rows, zero elsewhere, so a chain of MFMAs gives the
+//     partial scores of its groups apart and the group scales apply to the 32-bit results;
 //   scores  C[token][(h,g)] = sum_d (16 + code) q  - 24 sum_d q   (codes are fed as the bf16 16 + code: kv4.h; the
-//     accumulator starts at the constant), times the key's scale, summed over g by two quad permutes;
+//     accumulator starts at the constant), times the key's scale, summed over chains and, by quad permutes, columns;
 //   the score tiles' rows are chosen (kv4.h) so that a lane's 8 scores are the 8 tokens that it supplies to the
 //     PV product: P needs no exchange between lanes.  P s_v (rounded to bf16, as P itself would be) is its B
-//     operand in the same (h, g) columns, and of each result only the column of the row's own group is kept;
+//     operand in the same columns, one for each chain; of a result the columns of the row's own group are kept;
 //   O[d][(h,g)] = sum_t (16 + code) P s_v - 24 sum_t P s_v, the last sum by an MFMA with a matrix of ones so that it
 //     is over the same rounded values.
+// HPS is the smallest that holds the group's query heads (4, 8 or 16 at D = 128; 8 or 16 at 64; larger groups take
+// several workgroups): with the columns of 4 heads for every group size, 8 heads took two column sets, 210 registers
+// (2 waves per SIMD) and twice the softmax: 137 us at 64 x 8192 tokens, 64 / 8 heads x 128, instead of 110 (4.4 TB/s).
 // Statistics: running maximum per head with a deferred rescale (moves when a score exceeds it by 2^8), sums in
 // 32 bits.
 #include "kv4.h"
@@ -82,37 +85,45 @@ DEV_INLINE bf16x8 frag(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   return __builtin_bit_cast(bf16x8, make_uint4(a, b, c, d));
 }
 
-template <int D>
+// One record as a lane holds it: its chunks, and the scales of its column's group of every chain (so: the first's offset)
+template <int D, int NCH>
 struct Rec {
-  uint4 k[Kv4<D>::CH], v[Kv4<D>::CH], ks, vs;
+  uint4 k[Kv4<D>::CH], v[Kv4<D>::CH], ks[NCH], vs[NCH];
 };
-template <int D>
-DEV_INLINE void load_k(Rec<D>& t, const uint8_t* rec, int lane, int so) {
+template <int D, int NCH>
+DEV_INLINE void load_k(Rec<D, NCH>& t, const uint8_t* rec, int lane, int so) {
   using L = Kv4<D>;
 #pragma unroll
   for (int c = 0; c < L::CH; ++c) t.k[c] = *reinterpret_cast<const uint4*>(rec + L::KC + c * 1024 + lane * 16);
-  t.ks = *reinterpret_cast<const uint4*>(rec + L::KS + so);
+#pragma unroll
+  for (int c = 0; c < NCH; ++c) t.ks[c] = *reinterpret_cast<const uint4*>(rec + L::KS + so + c * (L::NG / NCH) * 16);
 }
-template <int D>
-DEV_INLINE void load_v(Rec<D>& t, const uint8_t* rec, int lane, int so) {
+template <int D, int NCH>
+DEV_INLINE void load_v(Rec<D, NCH>& t, const uint8_t* rec, int lane, int so) {
   using L = Kv4<D>;
 #pragma unroll
   for (int c = 0; c < L::CH; ++c) t.v[c] = *reinterpret_cast<const uint4*>(rec + L::VC + c * 1024 + lane * 16);
-  t.vs = *reinterpret_cast<const uint4*>(rec + L::VS + so);
+#pragma unroll
+  for (int c = 0; c < NCH; ++c) t.vs[c] = *reinterpret_cast<const uint4*>(rec + L::VS + so + c * (L::NG / NCH) * 16);
 }
 
 // The current token's codes put into the registers of the wave that read its record (token t of 32): the lanes
 // that hold its chunks take them from the lanes that quantised it, so nothing waits for the store.
-template <int D>
-DEV_INLINE void patch_rec(Rec<D>& x, int t, const Kv4Token& n, int lane) {
+template <int D, int NCH>
+DEV_INLINE void patch_rec(Rec<D, NCH>& x, int t, const Kv4Token& n, int lane) {
   using L = Kv4<D>;
-  const int r = lane & 15, q = lane >> 4, g = r % L::NG;
-  uint32_t w[L::NG], v[L::CH];
+  constexpr int NGC = L::NG / NCH;
+  const int r = lane & 15, q = lane >> 4, g = r % NGC;
+  uint32_t w[L::NG], v[L::CH], ks[NCH], vs[NCH];
 #pragma unroll
   for (int j = 0; j < L::NG; ++j) w[j] = __shfl(n.code, 8 * j + 2 * q, 64);
 #pragma unroll
-  for (int c = 0; c < L::CH; ++c) v[c] = __shfl(n.code, 32 + (D == 128 ? 2 * r + c : r), 64);
-  const uint32_t ks = __shfl(n.scale, 8 * g, 64), vs = __shfl(n.scale, 32 + 8 * g, 64);
+  for (int c = 0; c < L::CH; ++c) v[c] = __shfl(n.code, 32 + 16 * c + r, 64);
+#pragma unroll
+  for (int c = 0; c < NCH; ++c) {
+    ks[c] = __shfl(n.scale, 8 * (c * NGC + g), 64);
+    vs[c] = __shfl(n.scale, 32 + 8 * (c * NGC + g), 64);
+  }
   const int half = (t >> 2) & 1;
   if (r == 4 * (t >> 3) + (t & 3)) {
     if constexpr (D == 128) {
@@ -134,25 +145,29 @@ DEV_INLINE void patch_rec(Rec<D>& x, int t, const Kv4Token& n, int lane) {
     };
 #pragma unroll
     for (int c = 0; c < L::CH; ++c) put(x.v[c], v[c]);
-    put(x.ks, ks);
-    put(x.vs, vs);
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+      put(x.ks[c], ks[c]);
+      put(x.vs[c], vs[c]);
+    }
   }
 }
 
-// CS sets of 16 columns: HPS = 16 / NG query heads each (4 at D = 128, 8 at D = 64)
-template <int D, int CS, int NW>
+template <int D, int HPS, int NW>
 __global__ __launch_bounds__(64 * NW) void kv4_decode_kernel(Dec4Args a) {
   using L = Kv4<D>;
-  constexpr int NG = L::NG, NJ = L::NJ, HPS = 16 / NG;
-  __shared__ float red_m[NW][CS][16], red_l[NW][CS][16];
-  __shared__ float red_o[NW][CS][HPS][D];
+  constexpr int NG = L::NG, NGC = 16 / HPS, NCH = NG / NGC;
+  constexpr int NP = NGC == 1 ? 2 : 1;  // PV products a chunk of 64 d: its two groups are in one chain, or in two
+  static_assert(NGC <= NG && NGC * NCH == NG, "columns");
+  __shared__ float red_m[NW][16], red_l[NW][16];
+  __shared__ float red_o[NW][HPS][D];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int col = lane & 15, q = lane >> 4, g = col % NG, hc = col / NG;
-  const int G = a.H / a.KV, nhs = (G + HPS * CS - 1) / (HPS * CS);
+  const int col = lane & 15, q = lane >> 4, g = col % NGC, hc = col / NGC;
+  const int G = a.H / a.KV, nhs = (G + HPS - 1) / HPS;
   const int split = blockIdx.x % a.nsplit, item = blockIdx.x / a.nsplit;
   const int hs = item % nhs, kvh = item / nhs % a.KV, b = item / nhs / a.KV;
-  const int h0 = kvh * G + hs * HPS * CS, hn = min(HPS * CS, G - hs * HPS * CS);  // heads of this workgroup
+  const int h0 = kvh * G + hs * HPS, hn = min(HPS, G - hs * HPS);  // heads of this workgroup
   const Span sp = span_of<NW>(a, b);
   const int v0 = split * sp.per, v1 = min(sp.n, v0 + sp.per);
   if (v0 >= v1) {  // the join skips this part too
@@ -162,34 +177,34 @@ __global__ __launch_bounds__(64 * NW) void kv4_decode_kernel(Dec4Args a) {
     return;
   }
 
-  // q of column (h, g): values 32 g + 8 q + 0..7 of its head; zero in the other groups' MFMA steps
-  bf16x8 qf[CS][NG];
-  float bias[CS];
+  // q of column (h, g): in chain c values 32 (c NGC + g) + 8 q + 0..7 of its head; zero in the other groups' MFMA steps
+  bf16x8 qf[NG];
+  float bias[NCH];
 #pragma unroll
-  for (int s = 0; s < CS; ++s) {
-    const int h = s * HPS + hc;
+  for (int c = 0; c < NCH; ++c) {
     uint4 u = make_uint4(0, 0, 0, 0);
-    if (h < hn) u = *reinterpret_cast<const uint4*>(a.q + (long long)b * a.q_rs + (long long)(h0 + h) * D + 32 * g + 8 * q);
+    if (hc < hn)
+      u = *reinterpret_cast<const uint4*>(a.q + (long long)b * a.q_rs + (long long)(h0 + hc) * D + 32 * (c * NGC + g) + 8 * q);
     float f[8], t = 0.f;
     unpack8(u, f);
 #pragma unroll
     for (int e = 0; e < 8; ++e) t += f[e];
-    bias[s] = -24.0f * sum_q(t);
+    bias[c] = -24.0f * sum_q(t);
 #pragma unroll
-    for (int j = 0; j < NG; ++j) qf[s][j] = __builtin_bit_cast(bf16x8, j == g ? u : make_uint4(0, 0, 0, 0));
+    for (int j = 0; j < NGC; ++j) qf[c * NGC + j] = __builtin_bit_cast(bf16x8, j == g ? u : make_uint4(0, 0, 0, 0));
   }
   const bf16x8 ones = frag(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);
 
-  f32x4 acc[CS][NJ], accs[CS];
-  float m[CS], l[CS];
+  f32x4 acc[NP][L::CH][4], accs[NCH];
 #pragma unroll
-  for (int s = 0; s < CS; ++s) {
+  for (int p = 0; p < NP; ++p)
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) acc[s][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    accs[s] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    m[s] = -INFINITY;
-    l[s] = 0.f;
-  }
+    for (int c = 0; c < L::CH; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[p][c][i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int c = 0; c < NCH; ++c) accs[c] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;
   uint8_t* base = a.data + ((long long)b * a.KV + kvh) * a.tiles * L::REC;
   const int so = (q * NG + g) * 16;
   auto tile_of = [&](int v) { return v < sp.ts ? v : v - sp.ts + sp.tl; };
@@ -198,11 +213,11 @@ __global__ __launch_bounds__(64 * NW) void kv4_decode_kernel(Dec4Args a) {
   // The loads are unconditional (the last record is read once more): under a condition the compiler sinks them to
   // their use, which cost 294 instead of 193 us at 64 x 16384 tokens (32 / 8 heads x 128); two records in
   // registers spill their way to 594.
-  Rec<D> cur;
+  Rec<D, NCH> cur;
   {
     const uint8_t* rec = base + (long long)tile_of(min(v0 + wave, v1 - 1)) * L::REC;
-    load_k<D>(cur, rec, lane, so);
-    load_v<D>(cur, rec, lane, so);
+    load_k(cur, rec, lane, so);
+    load_v(cur, rec, lane, so);
   }
   // the wave of the last record quantises the current token, writes it and keeps its codes for that record
   const bool last = sp.append && v1 == sp.n && (sp.n - 1 - v0) % NW == wave;
@@ -216,11 +231,11 @@ __global__ __launch_bounds__(64 * NW) void kv4_decode_kernel(Dec4Args a) {
   auto record = [&](int v, bool more) __attribute__((always_inline)) {
     const int t0 = tile_of(v) * KV4_TILE;
     const uint8_t* next = base + (long long)tile_of(min(v + NW, v1 - 1)) * L::REC;
-    f32x4 c[CS][2];
+    f32x4 c[NCH][2];
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
 #pragma unroll
-      for (int s = 0; s < CS; ++s) c[s][half] = (f32x4){bias[s], bias[s], bias[s], bias[s]};
+      for (int ch = 0; ch < NCH; ++ch) c[ch][half] = (f32x4){bias[ch], bias[ch], bias[ch], bias[ch]};
 #pragma unroll
       for (int j = 0; j < NG; ++j) {
         uint32_t w;
@@ -228,122 +243,138 @@ __global__ __launch_bounds__(64 * NW) void kv4_decode_kernel(Dec4Args a) {
           w = j == 0 ? cur.k[half].x : j == 1 ? cur.k[half].y : j == 2 ? cur.k[half].z : cur.k[half].w;
         else
           w = half ? (j ? cur.k[0].w : cur.k[0].z) : (j ? cur.k[0].y : cur.k[0].x);
-        const bf16x8 kf = frag(pair16<0>(w), pair16<1>(w), pair16<2>(w), pair16<3>(w));
-#pragma unroll
-        for (int s = 0; s < CS; ++s) c[s][half] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[s][j], c[s][half], 0, 0, 0);
+        c[j / NGC][half] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+            frag(pair16<0>(w), pair16<1>(w), pair16<2>(w), pair16<3>(w)), qf[j], c[j / NGC][half], 0, 0, 0);
       }
     }
-    float x[CS][8];
-    {
+    float x[8];
+#pragma unroll
+    for (int ch = 0; ch < NCH; ++ch) {
       float ks[8];
-      unpack8(cur.ks, ks);
+      unpack8(cur.ks[ch], ks);
 #pragma unroll
-      for (int s = 0; s < CS; ++s)
+      for (int i = 0; i < 8; ++i) x[i] = ch ? x[i] + c[ch][i >> 2][i & 3] * ks[i] : c[ch][i >> 2][i & 3] * ks[i];
+    }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          x[s][i] = dpp_xor1(c[s][i >> 2][i & 3] * ks[i]);
-          if constexpr (NG == 4) x[s][i] = dpp_xor2(x[s][i]);
-        }
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (NGC >= 2) x[i] = dpp_xor1(x[i]);
+      if constexpr (NGC == 4) x[i] = dpp_xor2(x[i]);
     }
     __builtin_amdgcn_sched_barrier(0);
-    if (more) load_k<D>(cur, next, lane, so);
+    if (more) load_k(cur, next, lane, so);
     __builtin_amdgcn_sched_barrier(0);
-    float vs[8];
-    unpack8(cur.vs, vs);
     // tokens outside the length, or before the window and past the sinks: no weight, whatever their bytes hold
-    if (t0 + KV4_TILE > sp.len || (t0 < sp.lo && t0 + KV4_TILE > min(a.sinks, sp.lo))) {
+    const bool edge = t0 + KV4_TILE > sp.len || (t0 < sp.lo && t0 + KV4_TILE > min(a.sinks, sp.lo));
+    uint32_t hidden = 0;  // tokens without weight, one bit each
+    if (edge) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int t = t0 + 8 * q + i;
         const bool ok = t < sp.len && (t >= sp.lo || t < a.sinks);
-        vs[i] = ok ? vs[i] : 0.f;
-#pragma unroll
-        for (int s = 0; s < CS; ++s) x[s][i] = ok ? x[s][i] : -INFINITY;
+        hidden |= ok ? 0u : 1u << i;
+        x[i] = ok ? x[i] : -INFINITY;
       }
     }
-    bf16x8 pf[CS];
+    // c > 0: the maximum commutes with the scale
+    const float mt = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]))) * a.c;
+    if (__builtin_amdgcn_ballot_w64(mt > m + 8.0f) != 0) {
+      const float mn = fmaxf(m, max_q(mt));
+      const float al = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+      m = mn;
+      l *= al;
 #pragma unroll
-    for (int s = 0; s < CS; ++s) {
-      // c > 0: the maximum commutes with the scale
-      float mt = fmaxf(fmaxf(fmaxf(x[s][0], x[s][1]), fmaxf(x[s][2], x[s][3])),
-                       fmaxf(fmaxf(x[s][4], x[s][5]), fmaxf(x[s][6], x[s][7]))) * a.c;
-      if (__builtin_amdgcn_ballot_w64(mt > m[s] + 8.0f) != 0) {
-        const float mn = fmaxf(m[s], max_q(mt));
-        const float al = __builtin_amdgcn_exp2f(m[s] - (mn == -INFINITY ? 0.f : mn));
-        m[s] = mn;
-        l[s] *= al;
+      for (int p = 0; p < NP; ++p)
 #pragma unroll
-        for (int j = 0; j < NJ; ++j)
+        for (int ch = 0; ch < L::CH; ++ch)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) acc[s][j][i] *= al;
+          for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) accs[s][i] *= al;
-      }
-      const float mref = m[s] == -INFINITY ? 0.f : m[s];
+            for (int e = 0; e < 4; ++e) acc[p][ch][i][e] *= al;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[s][i], a.c, -mref));
-        l[s] += p;
-        x[s][i] = p * vs[i];
-      }
-      pf[s] = frag(pack_bf2(x[s][0], x[s][1]), pack_bf2(x[s][2], x[s][3]), pack_bf2(x[s][4], x[s][5]), pack_bf2(x[s][6], x[s][7]));
-      accs[s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, pf[s], accs[s], 0, 0, 0);
+      for (int ch = 0; ch < NCH; ++ch)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) accs[ch][e] *= al;
     }
-    auto pv = [&](int jj, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) __attribute__((always_inline)) {
+    const float mref = m == -INFINITY ? 0.f : m;
 #pragma unroll
-      for (int s = 0; s < CS; ++s)
-        acc[s][jj] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(frag(a0, a1, a2, a3), pf[s], acc[s][jj], 0, 0, 0);
-    };
+    for (int i = 0; i < 8; ++i) {
+      x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], a.c, -mref));
+      l += x[i];
+    }
+    bf16x8 pf[NCH];
 #pragma unroll
-    for (int c = 0; c < L::CH; ++c) {
-      const uint4 w = cur.v[c];
-      pv(4 * c + 0, pair16<0>(w.x), pair16<0>(w.y), pair16<0>(w.z), pair16<0>(w.w));
-      pv(4 * c + 1, pair16<1>(w.x), pair16<1>(w.y), pair16<1>(w.z), pair16<1>(w.w));
-      pv(4 * c + 2, pair16<2>(w.x), pair16<2>(w.y), pair16<2>(w.z), pair16<2>(w.w));
-      pv(4 * c + 3, pair16<3>(w.x), pair16<3>(w.y), pair16<3>(w.z), pair16<3>(w.w));
+    for (int ch = 0; ch < NCH; ++ch) {
+      float vs[8];
+      unpack8(cur.vs[ch], vs);
+      if (edge) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) vs[i] = (hidden >> i) & 1 ? 0.f : vs[i];
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) vs[i] *= x[i];
+      pf[ch] = frag(pack_bf2(vs[0], vs[1]), pack_bf2(vs[2], vs[3]), pack_bf2(vs[4], vs[5]), pack_bf2(vs[6], vs[7]));
+      accs[ch] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, pf[ch], accs[ch], 0, 0, 0);
+    }
+#pragma unroll
+    for (int ch = 0; ch < L::CH; ++ch) {
+      const uint4 w = cur.v[ch];
+      auto pv = [&](int i, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) __attribute__((always_inline)) {
+#pragma unroll
+        for (int p = 0; p < NP; ++p)  // the chain of group 2 ch + p
+          acc[p][ch][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(frag(a0, a1, a2, a3), pf[(2 * ch + p) / NGC], acc[p][ch][i], 0, 0, 0);
+      };
+      pv(0, pair16<0>(w.x), pair16<0>(w.y), pair16<0>(w.z), pair16<0>(w.w));
+      pv(1, pair16<1>(w.x), pair16<1>(w.y), pair16<1>(w.z), pair16<1>(w.w));
+      pv(2, pair16<2>(w.x), pair16<2>(w.y), pair16<2>(w.z), pair16<2>(w.w));
+      pv(3, pair16<3>(w.x), pair16<3>(w.y), pair16<3>(w.z), pair16<3>(w.w));
     }
     __builtin_amdgcn_sched_barrier(0);
-    if (more) load_v<D>(cur, next, lane, so);
+    if (more) load_v(cur, next, lane, so);
   };
   // the current token's record is peeled off: patching it inside the loop makes every record's loads wait
   int v = v0 + wave;
   for (const int ve = last ? v1 - 1 : v1; v < ve; v += NW) record(v, true);
   if (last) {
-    patch_rec<D>(cur, tok, fresh, lane);
+    patch_rec(cur, tok, fresh, lane);
     record(v, false);
   }
 
   // ---- join the waves: common maximum per column, then the sums in wave order
-#pragma unroll
-  for (int s = 0; s < CS; ++s) {
-    l[s] = sum_q(l[s]);
-    if (q == 0) red_m[wave][s][col] = m[s];
-  }
+  l = sum_q(l);
+  if (q == 0) red_m[wave][col] = m;
   __syncthreads();
-  const bool mine = g == (NG == 4 ? q : q >> 1);  // this lane's rows (d) are in its column's group
+  {
+    float M = red_m[0][col];
 #pragma unroll
-  for (int s = 0; s < CS; ++s) {
-    float M = red_m[0][s][col];
+    for (int w = 1; w < NW; ++w) M = fmaxf(M, red_m[w][col]);
+    const float al = __builtin_amdgcn_exp2f(m - (M == -INFINITY ? 0.f : M));
+    if (q == 0) red_l[wave][col] = l * al;
 #pragma unroll
-    for (int w = 1; w < NW; ++w) M = fmaxf(M, red_m[w][s][col]);
-    const float al = __builtin_amdgcn_exp2f(m[s] - (M == -INFINITY ? 0.f : M));
-    if (q == 0) red_l[wave][s][col] = l[s] * al;
-    if (mine) {
+    for (int ch = 0; ch < L::CH; ++ch) {
+      // this lane's rows r = 4 q + 0..3 are values of group 2 ch + (q >> 1): kept in that group's column
+      const bool mine = NGC == 1 || g == (2 * ch + (q >> 1)) % NGC;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int e = 0; e < 4; ++e) {
+        float o[4];
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) red_o[wave][s][hc][NJ * (4 * q + i) + j] = (acc[s][j][i] - 24.0f * accs[s][i]) * al;
+        for (int i = 0; i < 4; ++i) {
+          o[i] = (acc[0][ch][i][e] - 24.0f * accs[2 * ch / NGC][e]) * al;
+          if constexpr (NP == 2) o[i] = q >> 1 ? (acc[1][ch][i][e] - 24.0f * accs[2 * ch + 1][e]) * al : o[i];
+        }
+        if (mine)
+          *reinterpret_cast<float4*>(&red_o[wave][hc][64 * ch + 4 * (4 * q + e)]) = make_float4(o[0], o[1], o[2], o[3]);
+      }
     }
   }
   __syncthreads();
   for (int e = threadIdx.x; e < hn * D; e += 64 * NW) {
-    const int h = e / D, d = e % D, s = h / HPS, c = (h % HPS) * NG;
+    const int h = e / D, d = e % D, c = h * NGC;
     float o = 0.f, lt = 0.f, M = -INFINITY;
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
-      o += red_o[w][s][h % HPS][d];
-      lt += red_l[w][s][c];
-      M = fmaxf(M, red_m[w][s][c]);
+      o += red_o[w][h][d];
+      lt += red_l[w][c];
+      M = fmaxf(M, red_m[w][c]);
     }
     if (a.nsplit == 1) {
       a.out[(long long)b * a.o_rs + (long long)(h0 + h) * D + d] = f2bf(o / lt);
@@ -393,17 +424,14 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Dec4Args a) {
   }
 }
 
-// column sets a workgroup takes: enough for the group's query heads, at most 2 (8 heads at D = 128, 16 at 64);
-// larger groups take several workgroups
-int kv4_sets(int D, int G) { return G > (D == 128 ? 4 : 8) ? 2 : 1; }
 struct Plan {
-  int cs, nhs, nw, nsplit;
+  int hps, nhs, nw, nsplit;
 };
 Plan kv4_plan(int B, int H, int KV, int D, int max_len, int window, int sinks) {
   Plan p;
-  const int G = H / KV, hps = D == 128 ? 4 : 8;
-  p.cs = kv4_sets(D, G);
-  p.nhs = (G + hps * p.cs - 1) / (hps * p.cs);
+  const int G = H / KV;
+  p.hps = G <= 4 && D == 128 ? 4 : G <= 8 ? 8 : 16;
+  p.nhs = (G + p.hps - 1) / p.hps;
   const long long items = (long long)B * KV * p.nhs;
   long long vis = (max_len + KV4_TILE - 1) / KV4_TILE;
   if (window > 0) {
@@ -435,19 +463,25 @@ Plan kv4_plan(int B, int H, int KV, int D, int max_len, int window, int sinks) {
   return p;
 }
 
-template <int D, int CS, int NW>
+template <int D, int HPS, int NW>
 void launch(const Dec4Args& a, const Plan& p, hipStream_t stream) {
-  hipLaunchKernelGGL((kv4_decode_kernel<D, CS, NW>), dim3((unsigned)((long long)a.B * a.KV * p.nhs * p.nsplit)), dim3(64 * NW),
+  hipLaunchKernelGGL((kv4_decode_kernel<D, HPS, NW>), dim3((unsigned)((long long)a.B * a.KV * p.nhs * p.nsplit)), dim3(64 * NW),
                      0, stream, a);
   if (p.nsplit > 1)
     hipLaunchKernelGGL((kv4_join_kernel<D, NW>), dim3((unsigned)(a.B * a.H)), dim3(256), 0, stream, a);
 }
 template <int D>
 void launch_d(const Dec4Args& a, const Plan& p, hipStream_t stream) {
-  if (p.cs == 1)
-    p.nw == 8 ? launch<D, 1, 8>(a, p, stream) : launch<D, 1, 4>(a, p, stream);
+  if constexpr (D == 128) {
+    if (p.hps == 4) {
+      p.nw == 8 ? launch<D, 4, 8>(a, p, stream) : launch<D, 4, 4>(a, p, stream);
+      return;
+    }
+  }
+  if (p.hps == 8)
+    p.nw == 8 ? launch<D, 8, 8>(a, p, stream) : launch<D, 8, 4>(a, p, stream);
   else
-    p.nw == 8 ? launch<D, 2, 8>(a, p, stream) : launch<D, 2, 4>(a, p, stream);
+    p.nw == 8 ? launch<D, 16, 8>(a, p, stream) : launch<D, 16, 4>(a, p, stream);
 }
 
 }  // namespace

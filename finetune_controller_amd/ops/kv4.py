@@ -68,15 +68,14 @@ def _maps(D: int):
     codes, scales = KV4_TILE * D // 2, KV4_TILE * NG * 2
     g = torch.arange(NG)
     ks = codes + (blk[:, None] * NG + g) * 16 + i[:, None] * 2
-    # V: 16-byte chunk of lane (r, block): word p = tokens 2p | 2p + 1 (halves), values d0 + 0..3 each
+    # V: 16-byte chunk of lane (r, block): word p = tokens 2p | 2p + 1 (halves), values 64 c + 4 r + 0..3 each
     vb, vd = [], []
-    NJ = D // 16
-    for rr in range(16):
-        for quad in range(NJ // 4):
-            off = quad * 1024 + blk * 256 + rr * 16 + (i // 2) * 4 + (i % 2) * 2
+    for c in range(D // 64):
+        for rr in range(16):
+            off = c * 1024 + blk * 256 + rr * 16 + (i // 2) * 4 + (i % 2) * 2
             for b in range(2):
                 vb.append(codes + scales + off + b)
-                d0 = NJ * rr + 4 * quad + 2 * b
+                d0 = 64 * c + 4 * rr + 2 * b
                 vd.append((d0, d0 + 1))
     vs = ks + codes + scales
     return (torch.stack(kb, 1), torch.tensor(kd), ks, torch.stack(vb, 1), torch.tensor(vd), vs)

@@ -316,6 +316,20 @@ def test_decode_kernel_long(D, H, KV):
         _check(got, *_expected(qkv, k, v, lens, H, KV, D, D ** -0.5, window, sinks))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,H", [(128, 3), (128, 8), (128, 11), (64, 1), (64, 8), (64, 16)])
+def test_decode_kernel_many_short_sequences(D, H):
+    """More short sequences than workgroups of a round, every number of query heads a set of columns can hold."""
+    B, cap = 300, 96
+    lens = tuple((37 * b) % 91 for b in range(B))
+    qkv, k, v = _decode_case(B, H, 1, D, lens, cap, seed=31)
+    data = ops.kv4_alloc(B, cap, 1, D, device="cuda")
+    ops.kv4_store(data, k.cuda(), v.cuda(), torch.zeros(B, dtype=torch.int32, device="cuda"))
+    ln = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    got = ops.decode_attention_kv4(qkv.cuda(), data, ln, cap, H, 1, D)
+    _check(got, *_expected(qkv, k, v, lens, H, 1, D, D ** -0.5, 0, 0))
+
+
 @pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
 @pytest.mark.parametrize("max_len", [64, 120])
 def test_lengths_outside_the_bound(dev, max_len):
