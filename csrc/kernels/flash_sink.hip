@@ -70,8 +70,10 @@ DEV_INLINE float with_low_byte(uint32_t hi, uint32_t byte) {  // hi: the bf16 in
 // O is normalised by the sum of the weights as they were rounded for the PV product, so that the rounding of a row's
 // largest weights cancels (and 16 two-element dot products replace 32 adds a tile).  GRAD: a backward pass follows --
 // the output's low bits are kept, and the LSE of the unrounded weights.
-template <int D, bool GRAD>
-__global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void sink_fwd_kernel(FwdArgs a) {
+// GR = 2: two groups of WAVES waves take the block's key tiles in turn, each with its own buffers, and join their O, m, l
+// through LDS at the end -- for grids that leave most of the chip idle, where the chain of tiles is the time.
+template <int D, bool GRAD, int GR>
+__global__ __launch_bounds__(64 * WAVES * GR, 8 / WAVES) void sink_fwd_kernel(FwdArgs a) {
   constexpr int BQ = 32 * WAVES;
   constexpr int NCH = D / 8;           // 16-byte chunks per row
   constexpr int DSTEPS = D / 16;       // k-steps of the S MFMA
@@ -82,13 +84,16 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void sink_fwd_kernel(FwdArgs
   static_assert(NGT >= 1, "tile too small for the wave count");
   // K/V tiles double-buffered in four DISTINCT __shared__ objects: reading one does not make the
   // compiler drain the DMA still filling the other pair (LDS alias scopes)
-  __shared__ __attribute__((aligned(16))) char K0[TILE_BYTES];
-  __shared__ __attribute__((aligned(16))) char V0[TILE_BYTES];
-  __shared__ __attribute__((aligned(16))) char K1[TILE_BYTES];
-  __shared__ __attribute__((aligned(16))) char V1[TILE_BYTES];
+  __shared__ __attribute__((aligned(16))) char K0[GR * TILE_BYTES];
+  __shared__ __attribute__((aligned(16))) char V0[GR * TILE_BYTES];
+  __shared__ __attribute__((aligned(16))) char K1[GR * TILE_BYTES];
+  __shared__ __attribute__((aligned(16))) char V1[GR * TILE_BYTES];
 
   const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // provably wave-uniform -> scalar branches
+  const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);  // provably wave-uniform -> scalar branches
+  const int wave = GR == 1 ? wid : wid % WAVES, grp = GR == 1 ? 0 : wid / WAVES;
+  char *const K0g = K0 + grp * TILE_BYTES, *const V0g = V0 + grp * TILE_BYTES;
+  char *const K1g = K1 + grp * TILE_BYTES, *const V1g = V1 + grp * TILE_BYTES;
   const int hh = lane >> 5, lr = lane & 31;
   int qb, b, hq, kvh;
   decode_block(a, qb, b, hq, kvh);
@@ -150,7 +155,7 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void sink_fwd_kernel(FwdArgs
   float lw = 0.f;  // sum of the weights as rounded for the PV product
 
   __builtin_amdgcn_s_waitcnt(0x0F70);  // Q fragments (plain loads) retired before any DMA: vmcnt(0)
-  dma(tile_key(0), K0, V0);
+  if (GR == 1 || grp < ntiles) dma(tile_key(grp), K0g, V0g);
 
   // tr-read addressing (V^T A operand): 16-lane group gi = lane>>4 covers d cols [16*(gi&1), +16)
   // of the 32-wide d tile and key rows [16ks + 4*hh (+8), +4)
@@ -171,12 +176,12 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void sink_fwd_kernel(FwdArgs
 
   f32x16 s[2];   // S^T of the current tile, then its P (registers between the phases)
   bf16x8 pf[4];  // packed P^T operand of the PV MFMAs
-  // wait for tile t, barrier, then DMA tile t+1 into the slots that held tile t-1
+  // wait for tile t, barrier, then DMA the group's next tile into the slots that held the one before
   auto sync_tile = [&](const int t, char* Kn, char* Vn) __attribute__((always_inline)) {
     __builtin_amdgcn_s_waitcnt(0x0F70);  // this wave's pieces of tile t landed (vmcnt(0))
     __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
     __builtin_amdgcn_s_barrier();        // ... and everyone's
-    if (t + 1 < ntiles) dma(tile_key(t + 1), Kn, Vn);
+    if (t + GR < ntiles) dma(tile_key(t + GR), Kn, Vn);
   };
   // ---- phase A: S^T = K Q^T, two 32-key blocks
   auto phaseA = [&](const char* Kc) __attribute__((always_inline)) {
@@ -288,6 +293,7 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void sink_fwd_kernel(FwdArgs
   // wave passed this tile's barrier
   auto tile = [&](const int t, const char* Kc, const char* Vc, char* Kn, char* Vn) __attribute__((always_inline)) {
     sync_tile(t, Kn, Vn);
+    if (GR > 1 && t >= ntiles) return;  // (the groups meet at the same barriers)
     // a wave sees nothing of the tiles past its rows and before its window: with a short window they are many (341 us
     // instead of 362 at 4 x 4096 tokens, window 1024, 32 heads x 128; 0-1 % at 4096 of 8192 and 16384)
     const int kv0 = tile_key(t), qw = q0 + wave * 32;
@@ -296,9 +302,45 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void sink_fwd_kernel(FwdArgs
     phaseB1(t);
     phaseB2(Vc);
   };
-  for (int t = 0; t < ntiles; t += 2) {
-    tile(t, K0, V0, K1, V1);
-    if (t + 1 < ntiles) tile(t + 1, K1, V1, K0, V0);
+  const int steps = (ntiles + GR - 1) / GR;
+  for (int i = 0; i < steps; i += 2) {
+    tile(GR * i + grp, K0g, V0g, K1g, V1g);
+    if (i + 1 < steps) tile(GR * (i + 1) + grp, K1g, V1g, K0g, V0g);
+  }
+
+  // ---- join the groups: a lane holds the same row and elements in both; one shared object for each wave of a group
+  if constexpr (GR == 2) {
+    static_assert(WAVES == 4 && 64 * (DT * 16 + 3) * 4 <= GR * TILE_BYTES, "join buffers");
+    float* const jb = reinterpret_cast<float*>(wave == 0 ? K0 : wave == 1 ? V0 : wave == 2 ? K1 : V1);
+    __syncthreads();  // every wave is past its last tile
+    if (grp == 1) {
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<float4*>(jb + ((t * 4 + i) * 64 + lane) * 4) =
+              make_float4(o[t][4 * i], o[t][4 * i + 1], o[t][4 * i + 2], o[t][4 * i + 3]);
+      jb[DT * 1024 + lane] = m;
+      jb[DT * 1024 + 64 + lane] = lw;
+      jb[DT * 1024 + 128 + lane] = l;
+    }
+    __syncthreads();
+    if (grp == 1) return;
+    const float m1 = jb[DT * 1024 + lane], mn = fmaxf(m, m1), mref = mn == -INFINITY ? 0.f : mn;
+    const float a0 = __builtin_amdgcn_exp2f(m - mref), a1 = __builtin_amdgcn_exp2f(m1 - mref);
+    m = mn;
+    lw = lw * a0 + jb[DT * 1024 + 64 + lane] * a1;
+    l = l * a0 + jb[DT * 1024 + 128 + lane] * a1;
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float4 x = *reinterpret_cast<const float4*>(jb + ((t * 4 + i) * 64 + lane) * 4);
+        o[t][4 * i] = o[t][4 * i] * a0 + x.x * a1;
+        o[t][4 * i + 1] = o[t][4 * i + 1] * a0 + x.y * a1;
+        o[t][4 * i + 2] = o[t][4 * i + 2] * a0 + x.z * a1;
+        o[t][4 * i + 3] = o[t][4 * i + 3] * a0 + x.w * a1;
+      }
   }
 
   // ---- epilogue: normalise, store O (bf16) and LSE (natural log)
@@ -1083,6 +1125,12 @@ __global__ __launch_bounds__(256, 2) void sink_dq_kernel(BwdArgs a) {
   store_rows<DT>(op, dq, a.scale, hh, (a.dq_rs & 7) == 0);
 }
 
+template <int D, bool GRAD>
+void launch_fwd(const FwdArgs& a, long long blocks, bool two, hipStream_t stream) {
+  if (two) hipLaunchKernelGGL((sink_fwd_kernel<D, GRAD, 2>), dim3((unsigned)blocks), dim3(128 * WAVES), 0, stream, a);
+  else hipLaunchKernelGGL((sink_fwd_kernel<D, GRAD, 1>), dim3((unsigned)blocks), dim3(64 * WAVES), 0, stream, a);
+}
+
 }  // namespace
 
 extern "C" int ftc_sink_fwd(const void* q, const void* k, const void* v, void* o, void* olow, float* lse, int B, int S, int H, int KV,
@@ -1097,13 +1145,15 @@ extern "C" int ftc_sink_fwd(const void* q, const void* k, const void* v, void* o
             kv_rs, o_rs, B, S, H, KV, (S + BQ - 1) / BQ, scale * LOG2E, window < S ? window : S, sinks < S ? sinks : S};
   const long long blocks = (long long)a.nqb * B * H;
   if (blocks > 0x7fffffffLL) return -1;
-  if (D == 128) {
-    if (olow) hipLaunchKernelGGL((sink_fwd_kernel<128, true>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL((sink_fwd_kernel<128, false>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
-  } else {
-    if (olow) hipLaunchKernelGGL((sink_fwd_kernel<64, true>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL((sink_fwd_kernel<64, false>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
-  }
+  // One group where the blocks fill the chip, two where each has a CU to itself and more than two tiles (one group, two
+  // groups, us): 1 x 1000 tokens, 32 / 8 heads x 128 (256 blocks), window 999: 23.5, 19.9; 512: 20.1, 18.3; 16: 11.8, 11.7;
+  // 1 x 1001, 8 / 2 heads, window 256 (64 blocks): 15.0, 14.4; 320 blocks, window 512: 21.6, 21.5; 512 blocks: 35.7, 42.8;
+  // 1 x 100, 8 heads: 6.8, 7.7.
+  const bool two = blocks <= 256 && S > BQ;
+  if (D == 128)
+    olow ? launch_fwd<128, true>(a, blocks, two, stream) : launch_fwd<128, false>(a, blocks, two, stream);
+  else
+    olow ? launch_fwd<64, true>(a, blocks, two, stream) : launch_fwd<64, false>(a, blocks, two, stream);
   return (int)hipGetLastError();
 }
 

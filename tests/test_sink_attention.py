@@ -114,6 +114,7 @@ SHAPES = [  # B, S, H, KV, D, window, sinks
     (1, 700, 8, 1, 128, 200, 40),  # few key blocks: swept in parts
     (2, 530, 4, 2, 64, 530, 3),
     (16, 260, 32, 16, 64, 100, 5),  # many: each by one workgroup
+    (5, 260, 20, 4, 128, 150, 5),  # query blocks past one a compute unit
 ]
 
 
@@ -135,6 +136,21 @@ def test_kernels(B, S, H, KV, D, window, sinks):
     up, dn = (_definition(xd + t * e * d, do, B, S, H, KV, D, window, sinks, scale)[0] for t in (1, -1))
     diff = float(((up - dn) * do.double()).sum() / (2 * e))
     assert abs(float((g.double().cpu() * d).sum()) - diff) <= float((tg * d.abs()).sum()) + 1e-5 * abs(diff) + 1e-4
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,S,H,KV,D,window,sinks", [(1, 333, 4, 2, 128, 100, 4), (30, 333, 6, 3, 128, 100, 70),
+                                                     (2, 150, 4, 4, 80, 31, 3), (1, 1, 2, 1, 64, 5, 1)])
+def test_without_gradients(B, S, H, KV, D, window, sinks):
+    """The forward alone, from a wider projection into a padded output: the same values whether a backward may follow."""
+    qkv, do = _inputs(B, S, H, KV, D, seed=2)
+    wide = torch.cat([qkv, torch.full((B * S, 8), math.nan, dtype=BF)], 1).cuda()[:, :qkv.shape[1]]
+    wo, to, _, _ = _definition(qkv, do, B, S, H, KV, D, window, sinks, D ** -0.5)
+    with torch.no_grad():
+        o = ops.attention_packed(wide, B, S, H, KV, D, window=window, sinks=sinks, out_pad=8)
+    assert o.shape == (B * S, H * D) and o.stride(0) == H * D + 8 and not o.requires_grad
+    _close(o, wo, to)
+    assert torch.equal(o, ops.attention_packed(wide.requires_grad_(), B, S, H, KV, D, window=window, sinks=sinks).detach())
 
 
 @pytest.mark.gpu
