@@ -753,6 +753,7 @@ at::Tensor decode_attention_kv4(const at::Tensor& qkv_in, at::Tensor& data, cons
   need_value(max_len >= 1 && max_len <= (int64_t)c.tiles * 32, "decode_attention_kv4: max_len ", max_len,
              " outside the cache's 1..", (int64_t)c.tiles * 32);
   need_value(sinks >= 0, "decode_attention_kv4: sinks must not be negative, got ", sinks);
+  need_value(scale >= 0x1p-100 && scale <= 0x1p100, "decode_attention_kv4: scale must be positive and finite, got ", scale);
   c10::DeviceGuard guard(data.device());
   const at::Tensor qkv = rows16(qkv_in);
   auto out = at::empty({c.B, H * D}, qkv.options());

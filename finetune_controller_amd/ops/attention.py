@@ -397,6 +397,8 @@ def attention_packed(qkv: torch.Tensor, B: int, S: int, H: int, KV: int, D: int,
             raise ValueError(f"sinks must not be negative, got {sinks}")
         if not causal or docs is not None:
             raise ValueError("sinks: causal attention over one document per sequence only")
+        if not 2.0 ** -100 <= scale <= 2.0 ** 100:
+            raise ValueError(f"sinks: scale must be positive and finite, got {scale}")
         if not window or window <= 0:
             sinks = 0  # every earlier key is seen anyway
     if sinks and use_hip(qkv) and qkv.dtype == torch.bfloat16 and 0 < D <= 128 and B * S > 0:

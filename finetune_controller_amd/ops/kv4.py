@@ -218,8 +218,9 @@ def decode_attention_kv4(qkv: torch.Tensor, data: torch.Tensor, lens: torch.Tens
 
     ``qkv`` [B, (H+2KV)*D]: the current token's packed projection; its K / V rows are written at position
     ``lens - 1`` and attended to as they are held.  ``lens`` int32 [B] counts the current token; ``max_len``
-    (host int) bounds it (a longer sequence is attended to over its first ``max_len`` tokens and not written).  ``window`` > 0: the last ``window`` tokens and the first ``sinks`` are seen.  A
-    sequence of length 0 writes nothing and gives a zero row."""
+    (host int) bounds it (a longer sequence is attended to over its first ``max_len`` tokens and not written).
+    ``window`` > 0: the last ``window`` tokens and the first ``sinks`` are seen.  A sequence of length 0 writes
+    nothing and gives a zero row.  ``scale`` must be positive (1 / sqrt(D) by default)."""
     scale = scale if scale is not None else 1.0 / math.sqrt(D)
     if use_hip(qkv) and qkv.dtype == torch.bfloat16:
         return ext().decode_attention_kv4(qkv, data, lens, max_len, H, KV, D, scale, window or 0, sinks)
@@ -234,6 +235,8 @@ def decode_attention_kv4(qkv: torch.Tensor, data: torch.Tensor, lens: torch.Tens
         raise ValueError(f"decode_attention_kv4: max_len {max_len} outside the cache's 1..{cap}")
     if sinks < 0:
         raise ValueError(f"decode_attention_kv4: sinks must not be negative, got {sinks}")
+    if not 2.0 ** -100 <= scale <= 2.0 ** 100:
+        raise ValueError(f"decode_attention_kv4: scale must be positive and finite, got {scale}")
     window = max(0, int(window or 0))
     new = qkv[:, H * D:(H + 2 * KV) * D].unflatten(1, (2, KV * D))
     kv4_store(data, new[:, None, 0], new[:, None, 1], torch.where(lens <= max_len, lens - 1, lens - lens - 1))

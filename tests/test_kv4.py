@@ -217,6 +217,9 @@ def test_refusals(dev):
             ops.decode_attention_kv4(args[0], data, args[1], args[2], args[3], args[4], 64)
     with pytest.raises(ValueError, match="sinks"):
         ops.decode_attention_kv4(q, data, n, 64, 4, 2, 64, window=4, sinks=-1)
+    for scale in (0.0, -0.1, math.nan, math.inf):
+        with pytest.raises(ValueError, match="scale"):
+            ops.decode_attention_kv4(q, data, n, 64, 4, 2, 64, scale=scale)
     for bad in (dict(data=data.cpu()), dict(start=z.cpu()), dict(v=k.cpu())):
         if dev == "cuda":  # tensors of another device
             a = {**dict(data=data, v=k, start=z), **bad}

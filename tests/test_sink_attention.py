@@ -95,6 +95,9 @@ def test_refusals(dev):
     docs = ops.segments_from_eos(torch.zeros(1, 8, dtype=torch.long, device=dev), 5)
     with pytest.raises(ValueError, match="one document"):
         ops.attention_packed(qkv, 1, 8, 2, 1, 64, window=4, sinks=1, docs=docs)
+    for scale in (0.0, -0.1, math.nan, math.inf):
+        with pytest.raises(ValueError, match="scale"):
+            ops.attention_packed(qkv, 1, 8, 2, 1, 64, window=4, sinks=1, scale=scale)
 
 
 # ---------------------------------------------------------------- kernels
