@@ -27,6 +27,7 @@ struct Kv4 {
   static constexpr int CODES = KV4_TILE * D / 2;    // bytes
   static constexpr int SCALES = KV4_TILE * NG * 2;  // bytes
   static constexpr int REC = 2 * (CODES + SCALES);
+  static constexpr int WAVES = D == 128 ? 2 : 1;    // waves that write a record or read it back (kv4.hip)
   static constexpr int KC = 0, KS = CODES, VC = CODES + SCALES, VS = 2 * CODES + SCALES;
   // byte offset and shift of one value's code, and byte offset of its scale, within a record
   DEV_INLINE static void k_at(int t, int d, int* off, int* shift, int* soff) {
