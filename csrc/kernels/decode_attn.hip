@@ -1,5 +1,5 @@
-// Decode attention for generation: one new query token per sequence against its KV cache (GQA,
-// optional sliding window and sinks: the first keys stay visible), split over the key axis so a batch of long caches fills the 256 CUs.
+// Decode attention for generation: one new query token per sequence against its KV cache (GQA, optional sliding
+// window and sinks: the first keys stay visible), split over the key axis so a batch of long caches fills the 256 CUs.
 //
 // Decode is bound by HBM (every cached K/V byte is read once per generated token), so the layout is
 // chosen for coalesced 16-byte loads, not for MFMA:
