@@ -5,6 +5,7 @@
 // Every entry point validates device, dtype, contiguity and the shape assumptions of its kernel on
 // the host before launching -- a wrong shape must be a Python exception, never a GPU fault.
 #include <torch/extension.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime.h>
@@ -106,6 +107,12 @@ inline void check(int rc, const char* what) {
 inline void need(const at::Tensor& t, at::ScalarType dt, const char* name) {
   TORCH_CHECK(t.is_cuda(), name, " must be a GPU tensor");
   TORCH_CHECK(t.scalar_type() == dt, name, " has dtype ", t.scalar_type(), ", expected ", dt);
+}
+
+// An output or workspace on a tensor's device, past the dispatcher: 0.2 us less of the host for each, where a small call
+// takes 3 to 6 us.
+inline at::Tensor empty_on(const at::Tensor& like, at::IntArrayRef size, at::ScalarType dt) {
+  return at::detail::empty_cuda(size, dt, like.device(), c10::nullopt);
 }
 
 inline void need_rows(const at::Tensor& t, const char* name) {
@@ -546,7 +553,7 @@ void flash_bwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, co
 
 // ---------------- flash attention with a window and sinks (csrc/kernels/flash_sink.hip) ----------------
 // q, k, v are head-column views of one packed [B*S, (H+2KV)*D] projection (16-byte aligned rows), any S.
-// grad: the output's low bits (uint8) and the LSE are kept for the backward (empty tensors otherwise).
+// grad: the output's low bits (uint8) and the LSE are kept for the backward (undefined otherwise).
 inline void need_packed(const at::Tensor& qkv, int64_t B, int64_t S, int64_t W, const char* name) {
   need(qkv, at::kBFloat16, name);
   TORCH_CHECK(qkv.dim() == 2 && qkv.size(0) == B * S && qkv.size(1) >= W && qkv.stride(1) == 1 &&
@@ -566,12 +573,16 @@ std::vector<at::Tensor> sink_fwd(const at::Tensor& qkv, int64_t B, int64_t S, in
   need_packed(qkv, B, S, (H + 2 * KV) * D, "sink_fwd: qkv");
   TORCH_CHECK(pad >= 0 && pad % 8 == 0, "sink_fwd: pad must be a multiple of 8");
   c10::DeviceGuard guard(qkv.device());
-  auto obuf = at::empty({B * S, H * D + pad}, qkv.options());
+  auto obuf = empty_on(qkv, {B * S, H * D + pad}, at::kBFloat16);
   auto o = pad ? obuf.narrow(1, 0, H * D) : obuf;
-  auto lse = at::empty({grad ? B : 0, H, S}, qkv.options().dtype(at::kFloat));
-  auto olow = at::empty({grad ? B * S : 0, H * D}, qkv.options().dtype(at::kByte));
+  at::Tensor lse, olow;
+  if (grad) {
+    lse = empty_on(qkv, {B, H, S}, at::kFloat);
+    olow = empty_on(qkv, {B * S, H * D}, at::kByte);
+  }
   const auto* p = static_cast<const uint16_t*>(qkv.data_ptr());
-  check(ftc_sink_fwd(p, p + H * D, p + (H + KV) * D, o.data_ptr(), grad ? olow.data_ptr() : nullptr, lse.data_ptr<float>(), (int)B, (int)S, (int)H, (int)KV,
+  check(ftc_sink_fwd(p, p + H * D, p + (H + KV) * D, o.data_ptr(), grad ? olow.data_ptr() : nullptr,
+                     grad ? lse.data_ptr<float>() : nullptr, (int)B, (int)S, (int)H, (int)KV,
                      (int)D, qkv.stride(0), qkv.stride(0), o.stride(0), (float)scale, (int)std::min(window, S),
                      (int)std::min(sinks, S), cur_stream()),
         "sink_fwd");
@@ -618,11 +629,10 @@ at::Tensor sink_bwd(const at::Tensor& qkv, const at::Tensor& o, const at::Tensor
     }
   }
   c10::DeviceGuard guard(qkv.device());
-  auto buf = at::empty({B * S, W + pad}, qkv.options());
+  auto buf = empty_on(qkv, {B * S, W + pad}, at::kBFloat16);
   auto dqkv = pad ? buf.narrow(1, 0, W) : buf;
   const int win = (int)std::min(window, S), snk = (int)std::min(sinks, S);
-  auto ws = at::empty({ftc_sink_bwd_workspace((int)B, (int)S, (int)H, (int)KV, (int)D, win, snk)},
-                      qkv.options().dtype(at::kFloat));
+  auto ws = empty_on(qkv, {ftc_sink_bwd_workspace((int)B, (int)S, (int)H, (int)KV, (int)D, win, snk)}, at::kFloat);
   const auto* p = static_cast<const uint16_t*>(qkv.data_ptr());
   auto* g = static_cast<uint16_t*>(dqkv.data_ptr());
   check(ftc_sink_bwd(p, p + H * D, p + (H + KV) * D, o.data_ptr(), olow.data_ptr(), dout.data_ptr(), lse.data_ptr<float>(), g,
@@ -731,8 +741,7 @@ std::tuple<at::Tensor, at::Tensor> kv4_load(const at::Tensor& data, const at::Te
   need_index(start, data, "kv4_load: start");
   need_value(n >= 0 && n < (1LL << 30), "kv4_load: n must not be negative, got ", n);
   c10::DeviceGuard guard(data.device());
-  auto k = at::empty({c.B, n, c.KV * D}, data.options().dtype(at::kBFloat16));
-  auto v = at::empty_like(k);
+  auto k = empty_on(data, {c.B, n, c.KV * D}, at::kBFloat16), v = empty_on(data, {c.B, n, c.KV * D}, at::kBFloat16);
   if (n > 0)
     check(ftc_kv4_load(data.data_ptr(), k.data_ptr(), v.data_ptr(), start.data_ptr<int>(), c.B, c.KV, (int)D, (int)n,
                        c.tiles, cur_stream()),
@@ -756,12 +765,12 @@ at::Tensor decode_attention_kv4(const at::Tensor& qkv_in, at::Tensor& data, cons
   need_value(scale >= 0x1p-100 && scale <= 0x1p100, "decode_attention_kv4: scale must be positive and finite, got ", scale);
   c10::DeviceGuard guard(data.device());
   const at::Tensor qkv = rows16(qkv_in);
-  auto out = at::empty({c.B, H * D}, qkv.options());
+  auto out = empty_on(data, {c.B, H * D}, at::kBFloat16);
   const int win = (int)std::min<int64_t>(std::max<int64_t>(window, 0), 1 << 30);
   const int snk = (int)std::min<int64_t>(sinks, 1 << 30);
   const int64_t wsf = ftc_kv4_decode_workspace_floats(c.B, (int)H, (int)KV, (int)D, (int)max_len, win, snk);
   at::Tensor ws;
-  if (wsf > 0) ws = at::empty({wsf}, qkv.options().dtype(at::kFloat));
+  if (wsf > 0) ws = empty_on(data, {wsf}, at::kFloat);
   check(ftc_kv4_decode(qkv.data_ptr(), data.data_ptr(), lens.data_ptr<int>(), out.data_ptr(),
                        wsf > 0 ? ws.data_ptr<float>() : nullptr, c.B, (int)H, (int)KV, (int)D, c.tiles, (int)max_len,
                        qkv.stride(0), out.stride(0), (float)scale, win, snk, cur_stream()),

@@ -401,7 +401,11 @@ def attention_packed(qkv: torch.Tensor, B: int, S: int, H: int, KV: int, D: int,
             raise ValueError(f"sinks: scale must be positive and finite, got {scale}")
         if not window or window <= 0:
             sinks = 0  # every earlier key is seen anyway
-    if sinks and use_hip(qkv) and qkv.dtype == torch.bfloat16 and 0 < D <= 128 and B * S > 0:
+    if sinks and B * S == 0:
+        return qkv[:, :H * D].clone()  # (the library's attention launches an empty grid for no rows)
+    if sinks and use_hip(qkv) and qkv.dtype == torch.bfloat16:
+        if D > 128:
+            raise ValueError(f"sinks: head_dim up to 128 in bf16, got {D}")
         if kernel_head_dim(D) == D and not (qkv.requires_grad and torch.is_grad_enabled()):
             return ext().sink_fwd(_rows16(qkv), B, S, H, KV, D, scale, int(window), int(sinks), out_pad, False)[0]
         return _FlashSinks.apply(qkv, B, S, H, KV, D, int(window), int(sinks), scale, out_pad, grad_pad, rope_grad,

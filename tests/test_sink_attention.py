@@ -95,9 +95,21 @@ def test_refusals(dev):
     docs = ops.segments_from_eos(torch.zeros(1, 8, dtype=torch.long, device=dev), 5)
     with pytest.raises(ValueError, match="one document"):
         ops.attention_packed(qkv, 1, 8, 2, 1, 64, window=4, sinks=1, docs=docs)
+    if dev == "cuda":
+        with pytest.raises(ValueError, match="head_dim"):
+            ops.attention_packed(torch.zeros(8, 4 * 136, dtype=BF, device=dev), 1, 8, 2, 1, 136, window=4, sinks=1)
     for scale in (0.0, -0.1, math.nan, math.inf):
         with pytest.raises(ValueError, match="scale"):
             ops.attention_packed(qkv, 1, 8, 2, 1, 64, window=4, sinks=1, scale=scale)
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("B,S", [(0, 4), (2, 0)])
+def test_nothing_to_attend_to(dev, B, S):
+    x = torch.zeros(B * S, 4 * 64, dtype=BF, device=dev, requires_grad=True)
+    o = ops.attention_packed(x, B, S, 2, 1, 64, window=3, sinks=1)
+    (g,) = torch.autograd.grad(o.sum(), x)
+    assert o.shape == (0, 128) and g.shape == x.shape
 
 
 # ---------------------------------------------------------------- kernels
