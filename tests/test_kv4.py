@@ -357,6 +357,39 @@ def test_lengths_outside_the_bound(dev, max_len):
 
 
 @pytest.mark.gpu
+def test_a_cache_past_32_bit_offsets():
+    """4.8 GB, 2^21 tokens: the far ends are written, read back and attended to as the same tokens in a small cache are."""
+    B, H, KV, D, cap, small = 2, 16, 8, 128, 2 ** 21, 320
+    window, sinks, tail = 100, 8, 150
+    lens, short = (cap, cap - 52), (small, small - 52)
+    qkv, k, v = _decode_case(B, H, KV, D, None, small, seed=41)
+    dev = dict(dtype=torch.int32, device="cuda")
+    data = ops.kv4_alloc(B, cap, KV, D, device="cuda")
+    assert data.numel() > 2 ** 32
+    i = torch.stack([torch.arange(n - tail, n) for n in short])  # the small cache's last rows, put at the end
+    far = [torch.stack([t[b, i[b]] for b in range(B)]).cuda() for t in (k, v)]
+    at = torch.tensor([n - tail for n in lens], **dev)
+    ops.kv4_store(data, *far, at)
+    for g, w in zip(ops.kv4_load(data, at, tail, D), far):
+        # (read back as bf16: the held values, 12 significant bits, rounded once)
+        assert torch.equal(g.cpu(), _codes_of(w.cpu().unflatten(-1, (KV, D))).flatten(-2).to(BF))
+    ops.kv4_store(data, k[:, :sinks].cuda(), v[:, :sinks].cuda(), torch.zeros(B, **dev))
+    got = ops.decode_attention_kv4(qkv.cuda(), data, torch.tensor(lens, **dev), cap, H, KV, D, window=window, sinks=sinks)
+    _check(got, *_expected(qkv, k, v, short, H, KV, D, D ** -0.5, window, sinks))
+    # the whole length: keys of zero weigh alike, and only the last rows' values are not zero
+    data.zero_()
+    ops.kv4_store(data, torch.zeros_like(far[0]), far[1], at)
+    flat = qkv.clone()
+    flat[:, H * D:(H + KV) * D] = 0
+    got = ops.decode_attention_kv4(flat.cuda(), data, torch.tensor(lens, **dev), cap, H, KV, D)
+    V = _codes_of(far[1].cpu().unflatten(-1, (KV, D)))  # [B, tail, KV, D]
+    V[:, -1] = _codes_of(flat[:, (H + KV) * D:].view(B, KV, D))
+    n = torch.tensor(lens, dtype=torch.float64)[:, None, None]
+    want, pv = V.sum(1) / n, V.abs().sum(1) / n
+    _check(got, *(t.repeat_interleave(H // KV, 1).flatten(1) for t in (want, pv)))
+
+
+@pytest.mark.gpu
 def test_decode_step_on_a_stream_and_in_a_graph():
     """The same step eagerly, on a side stream and replayed from a graph with growing lengths."""
     B, H, KV, D, cap = 3, 8, 2, 128, 200

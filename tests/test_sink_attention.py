@@ -212,6 +212,26 @@ def test_expanded_and_single_row_gradients():
 
 
 @pytest.mark.gpu
+def test_projections_past_32_bit_offsets():
+    """4.8 GB of rows: the last sequence's last rows are those of a short sequence of what they see."""
+    B, S, D, window, sinks, tail = 3, 2 ** 22, 64, 64, 4, 100
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(B * S, 3 * D, generator=g, device="cuda", dtype=BF)
+    do = torch.randn(B * S, D, generator=g, device="cuda", dtype=BF)
+    assert x.numel() * 2 > 2 ** 32
+    near = torch.cat([torch.arange(sinks), torch.arange(S - tail - window, S)]) + (B - 1) * S
+    wo, to, wg, tg = _definition(x[near.cuda()].cpu(), do[near.cuda()].cpu(), 1, near.numel(), 1, 1, D, window, sinks, D ** -0.5)
+    x.requires_grad_()
+    o = ops.attention_packed(x, B, S, 1, 1, D, window=window, sinks=sinks)
+    (gx,) = torch.autograd.grad(o, x, do)
+    _close(o[-tail:], wo[-tail:], to[-tail:])
+    _close(gx[-tail:], wg[-tail:], tg[-tail:])
+    # and the first sequence's rows before any window is left
+    wo, to, _, _ = _definition(x.detach()[:window].cpu(), do[:window].cpu(), 1, window, 1, 1, D, window, sinks, D ** -0.5)
+    _close(o[:window], wo, to)
+
+
+@pytest.mark.gpu
 def test_rope_handoff():
     """The backward takes RoPE's inverse rotation into its epilogues (rows past a tile, positions given)."""
     B, S, H, KV, D, window, sinks = 2, 290, 2, 1, 128, 64, 4
