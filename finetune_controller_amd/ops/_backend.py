@@ -79,6 +79,11 @@ def ext():
     return load_ext(required=True)
 
 
+def has_tangent(t: torch.Tensor) -> bool:
+    """``t`` carries a forward-mode derivative (``torch.autograd.forward_ad``), with or without ``requires_grad``."""
+    return torch.autograd.forward_ad.unpack_dual(t).tangent is not None
+
+
 def stream_ptr(device: torch.device | None = None) -> int:
     """Raw hipStream_t of the current torch stream (kernels launch on it)."""
     return torch.cuda.current_stream(device).cuda_stream

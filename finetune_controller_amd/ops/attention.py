@@ -26,7 +26,7 @@ from dataclasses import dataclass
 import torch
 import torch.nn.functional as F
 
-from ._backend import ext, use_hip
+from ._backend import ext, has_tangent, use_hip
 from .linear import gate_wgrad_stream as _gate_dw
 
 
@@ -406,7 +406,8 @@ def attention_packed(qkv: torch.Tensor, B: int, S: int, H: int, KV: int, D: int,
     if sinks and use_hip(qkv) and qkv.dtype == torch.bfloat16:
         if D > 128:
             raise ValueError(f"sinks: head_dim up to 128 in bf16, got {D}")
-        if kernel_head_dim(D) == D and not (qkv.requires_grad and torch.is_grad_enabled()):
+        # without derivatives: past autograd (a tangent goes to it, and is refused there)
+        if kernel_head_dim(D) == D and not (qkv.requires_grad and torch.is_grad_enabled()) and not has_tangent(qkv):
             return ext().sink_fwd(_rows16(qkv), B, S, H, KV, D, scale, int(window), int(sinks), out_pad, False)[0]
         return _FlashSinks.apply(qkv, B, S, H, KV, D, int(window), int(sinks), scale, out_pad, grad_pad, rope_grad,
                                  torch.is_grad_enabled())

@@ -298,3 +298,31 @@ def test_everything_in_the_window_equals_causal_attention():
         (g,) = torch.autograd.grad(o, x, do)
         _close(o, wo, to)
         _close(g, wg, tg)
+
+
+# ---------------------------------------------------------------- derivatives that the kernels do not have
+class _StubKernels:
+    """The extension's forward without a GPU: an output and no derivative, as a kernel gives it."""
+
+    def sink_fwd(self, qkv, B, S, H, KV, D, scale, window, sinks, out_pad, grad):
+        return qkv.new_zeros(B * S, H * D), None, None
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("D", [64, 48])
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_is_refused(dev, D, grad, monkeypatch):
+    """A tensor that carries a tangent is refused: it never comes back as an output without one."""
+    from torch.autograd import forward_ad
+
+    from finetune_controller_amd.ops import attention
+
+    if dev == "cpu":
+        monkeypatch.setattr(attention, "use_hip", lambda t: True)
+        monkeypatch.setattr(attention, "ext", _StubKernels)
+    x = torch.randn(6, 4 * D, dtype=BF, device=dev).requires_grad_(grad)
+    for mode in (torch.enable_grad, torch.no_grad):
+        with forward_ad.dual_level(), mode(), pytest.raises(NotImplementedError):
+            ops.attention_packed(forward_ad.make_dual(x, torch.ones_like(x)), 1, 6, 2, 1, D, window=3, sinks=1)
+        with forward_ad.dual_level(), torch.no_grad():  # the level alone refuses nothing
+            assert ops.attention_packed(x, 1, 6, 2, 1, D, window=3, sinks=1).shape == (6, 2 * D)
