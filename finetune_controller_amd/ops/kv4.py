@@ -25,7 +25,7 @@ import math
 
 import torch
 
-from ._backend import ext, use_hip
+from ._backend import ext, has_tangent, use_hip
 from .decode import KVCache, visible_keys
 
 KV4_TILE = 32   # tokens per record
@@ -220,10 +220,14 @@ def decode_attention_kv4(qkv: torch.Tensor, data: torch.Tensor, lens: torch.Tens
     ``lens - 1`` and attended to as they are held.  ``lens`` int32 [B] counts the current token; ``max_len``
     (host int) bounds it (a longer sequence is attended to over its first ``max_len`` tokens and not written).
     ``window`` > 0: the last ``window`` tokens and the first ``sinks`` are seen.  A sequence of length 0 writes
-    nothing and gives a zero row.  ``scale`` must be positive (1 / sqrt(D) by default)."""
+    nothing and gives a zero row.  ``scale`` must be positive (1 / sqrt(D) by default).  For inference: the output has
+    no gradient, and a ``qkv`` with a forward-mode tangent is refused."""
+    if has_tangent(qkv):
+        raise NotImplementedError("decode_attention_kv4 has no derivative")
     scale = scale if scale is not None else 1.0 / math.sqrt(D)
     if use_hip(qkv) and qkv.dtype == torch.bfloat16:
         return ext().decode_attention_kv4(qkv, data, lens, max_len, H, KV, D, scale, window or 0, sinks)
+    qkv = qkv.detach()
     B, nkv, cap = _check_cache(data, D)
     if nkv != KV or KV < 1 or H < KV or H % KV:
         raise ValueError(f"decode_attention_kv4: {H} query / {KV} kv heads on a cache of {nkv}")

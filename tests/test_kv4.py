@@ -424,3 +424,30 @@ def test_decode_step_on_a_stream_and_in_a_graph():
         assert torch.equal(out, want[i]), i
         lens += 1
     assert torch.equal(data, eager)
+
+
+class _StubKernels:
+    """The extension's decode attention without a GPU: an output and no derivative, as a kernel gives it."""
+
+    def decode_attention_kv4(self, qkv, data, lens, max_len, H, KV, D, scale, window, sinks):
+        return qkv.detach().new_zeros(qkv.shape[0], H * D)
+
+
+@pytest.mark.parametrize("dev", ["cpu", "kernels without a gpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_decode_attention_has_no_derivative(dev, monkeypatch):
+    """Both paths alike: an output that requires no grad, and a tensor with a tangent is refused."""
+    from torch.autograd import forward_ad
+
+    if dev == "kernels without a gpu":
+        monkeypatch.setattr(kv4, "use_hip", lambda t: True)
+        monkeypatch.setattr(kv4, "ext", _StubKernels)
+        dev = "cpu"
+    data = ops.kv4_alloc(2, 32, 1, 64, device=dev)
+    lens = torch.tensor([1, 5], dtype=torch.int32, device=dev)
+    x = _rows(2, 4 * 64).to(dev).requires_grad_()
+    assert not ops.decode_attention_kv4(x, data, lens, 32, 2, 1, 64).requires_grad
+    before = data.clone()
+    for y in (x, x.detach()):
+        with forward_ad.dual_level(), pytest.raises(NotImplementedError, match="derivative"):
+            ops.decode_attention_kv4(forward_ad.make_dual(y, torch.ones_like(y)) * 2, data, lens, 32, 2, 1, 64)
+    assert torch.equal(before, data)
