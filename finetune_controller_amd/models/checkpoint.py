@@ -7,7 +7,8 @@ flattens sub-directories to basenames when zipping/presigning
 unique names:
 
 * LoRA / QLoRA: ``adapter_config.json`` (PEFT) + ``adapter_model.safetensors`` + ``adapter_model.pt``
-  (same tensors; ``.pt`` is matched by the reference's default patterns, safetensors by ours);
+  (same tensors; ``.pt`` is matched by the reference's default patterns, safetensors by ours), and
+  ``adapter_attention.json``: the window and sinks it was trained with (PEFT's file holds PEFT's keys only);
 * full fine-tune: ``config.json`` + ``model-0000i-of-0000n.safetensors`` shards +
   ``model.safetensors.index.json`` in Hugging Face naming (+ nothing pickled);
 * resume: ``checkpoint_step{N}.pt`` (trainable tensors + optimizer flat state + data cursor),
@@ -29,6 +30,7 @@ from .lora import LoRAConfig
 _log = logging.getLogger("ftc.checkpoint")
 
 PEFT_PREFIX = "base_model.model."
+ADAPTER_ATTENTION = "adapter_attention.json"
 
 _LLAMA_SEG_MODULE = {"q_proj": "self_attn", "k_proj": "self_attn", "v_proj": "self_attn", "o_proj": "self_attn",
                      "gate_proj": "mlp", "up_proj": "mlp", "down_proj": "mlp"}
@@ -65,6 +67,7 @@ def _atomic(path: str, write):
 
 
 def save_adapter(model, out_dir: str, base_model_name: str, lora: LoRAConfig, write_pt: bool = True) -> list[str]:
+    """Write the adapter; returns the PEFT files (``adapter_attention.json`` beside them is this framework's own)."""
     os.makedirs(out_dir, exist_ok=True)
     sd = adapter_state_dict(model)
     files = []
@@ -79,7 +82,23 @@ def save_adapter(model, out_dir: str, base_model_name: str, lora: LoRAConfig, wr
     with open(p, "w") as f:
         json.dump(lora.to_peft(base_model_name), f, indent=2)
     files.append(p)
+    with open(os.path.join(out_dir, ADAPTER_ATTENTION), "w") as f:
+        json.dump({"sliding_window": model.cfg.sliding_window, "attention_sinks": model.cfg.attention_sinks}, f)
     return files
+
+
+def adapter_attention(path: str) -> tuple[int, int]:
+    """``(sliding_window, attention_sinks)`` that the adapter directory ``path`` was trained with, from the file that
+    ``save_adapter`` writes or else the trainer's ``training_config.json``; (-1, -1) = not known (the model's own)."""
+    for name in (ADAPTER_ATTENTION, "training_config.json"):
+        f = os.path.join(path, name)
+        if os.path.exists(f):
+            with open(f) as h:
+                rec = json.load(h)
+            rec = rec.get("model", {}) if name != ADAPTER_ATTENTION else rec
+            if "sliding_window" in rec:
+                return int(rec["sliding_window"]), int(rec.get("attention_sinks", 0))
+    return -1, -1
 
 
 @torch.no_grad()

@@ -174,11 +174,19 @@ def main(argv=None) -> int:
     ap.add_argument("--top-p", type=float, default=1.0)
     ap.add_argument("--seed", type=int, default=0)
     ap.add_argument("--kv-bits", type=int, default=16, choices=[4, 16], help="4: hold the KV cache in 4 bits")
-    ap.add_argument("--sliding-window", type=int, default=-1, help="attention window (-1: the model's, 0: full causal)")
+    ap.add_argument("--sliding-window", type=int, default=-1,
+                    help="attention window (-1: what the adapter was trained with, or the model's; 0: full causal)")
     ap.add_argument("--attention-sinks", type=int, default=-1,
-                    help="first tokens that stay visible beside the window (-1: the model's)")
+                    help="first tokens that stay visible beside the window (-1: the adapter's or the model's)")
     a = ap.parse_args(argv)
-    cfg = get_config(a.model, a.sliding_window, a.attention_sinks)
+    window, sinks = a.sliding_window, a.attention_sinks
+    if a.adapter:
+        trained = ckpt.adapter_attention(a.adapter)
+        if sinks < 0 and window != 0:
+            sinks = trained[1]
+        if window < 0:
+            window = trained[0]
+    cfg = get_config(a.model, window, sinks)
     dev = torch.device("cuda" if torch.cuda.device_count() > 0 and torch.cuda.is_available() else "cpu")
     lora = None
     if a.adapter:

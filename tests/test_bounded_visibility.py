@@ -261,3 +261,41 @@ def test_sequence_parallel_with_sinks_matches_a_single_process(tmp_path):
     assert abs((res[0]["loss"] + res[1]["loss"]) / 2 - ref_loss) < 1e-5 * abs(ref_loss)
     torch.testing.assert_close(res[0]["grad"] / 2, ref, atol=1e-6 * ref.abs().max().item(), rtol=1e-4)
     assert not math.isnan(ref_loss)
+
+
+@pytest.mark.parametrize("model,trained", [("llama-tiny", (16, 3)), ("mistral-tiny", (0, -1)), ("mistral-tiny", (-1, 2)),
+                                           ("llama-tiny", (-1, -1))])
+def test_an_adapter_keeps_the_attention_it_was_trained_with(tmp_path, monkeypatch, model, trained):
+    """Generation from a LoRA adapter without flags sees what training saw; flags still replace it."""
+    from finetune_controller_amd.models import checkpoint as ckpt
+    from finetune_controller_amd.models import generate as gen
+
+    tr = Trainer(TrainConfig(model=model, method="lora", batch_size=1, seq_len=32, synthetic=True, max_steps=1, resume=False,
+                             checkpoint_path=str(tmp_path / "out"), device="cpu", sliding_window=trained[0],
+                             attention_sinks=trained[1]))
+    want = (tr.cfg.sliding_window, tr.cfg.attention_sinks)
+    tr.run()
+    ckpt.save_adapter(tr.model, str(tmp_path / "saved"), model, tr.lora)  # by itself, without the trainer's records
+    tr.close()
+    used = []
+
+    def seen(m, *a, **k):
+        used.append((m.cfg.sliding_window, m.cfg.attention_sinks))
+        return [[5]]
+
+    monkeypatch.setattr(gen, "generate", seen)
+    (tmp_path / "older").mkdir()  # an adapter that has the trainer's record only
+    for f in ("adapter_config.json", "adapter_model.safetensors", "training_config.json"):
+        (tmp_path / "older" / f).write_bytes((tmp_path / "out" / f).read_bytes())
+    for d in ("out", "saved", "older"):
+        assert gen.main(["--model", model, "--adapter", str(tmp_path / d), "--prompt", "a"]) == 0
+        assert used.pop() == want, d
+    flags = ["--sliding-window", "9", "--attention-sinks", "1"]
+    assert gen.main(["--model", model, "--adapter", str(tmp_path / "out"), "--prompt", "a", *flags]) == 0
+    assert used.pop() == (9, 1)
+    conf = json.load(open(tmp_path / "out" / "adapter_config.json"))
+    assert not {"sliding_window", "attention_sinks"} & set(conf)  # the PEFT file holds PEFT's keys only
+    (tmp_path / "older" / "training_config.json").unlink()  # neither record: the model's own
+    assert gen.main(["--model", model, "--adapter", str(tmp_path / "older"), "--prompt", "a"]) == 0
+    own = get_config(model)
+    assert used.pop() == (own.sliding_window, own.attention_sinks)
