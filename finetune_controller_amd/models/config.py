@@ -154,7 +154,8 @@ PRESETS: dict[str, ModelConfig] = {
 
 
 def get_config(name_or_path: str, sliding_window: int = -1, attention_sinks: int = -1) -> ModelConfig:
-    """A preset or an HF ``config.json``; ``sliding_window`` / ``attention_sinks`` >= 0 replace the model's own."""
+    """A preset or an HF ``config.json``; ``sliding_window`` / ``attention_sinks`` >= 0 replace the model's own (a
+    ``sliding_window`` of 0, full causal attention, takes the model's sinks with it)."""
     if name_or_path in PRESETS:
         cfg = dataclasses.replace(PRESETS[name_or_path])
     else:
@@ -164,6 +165,8 @@ def get_config(name_or_path: str, sliding_window: int = -1, attention_sinks: int
         cfg.sliding_window = sliding_window
     if attention_sinks >= 0:
         cfg.attention_sinks = attention_sinks
+    elif sliding_window == 0:
+        cfg.attention_sinks = 0
     if cfg.family != "llama" and (cfg.sliding_window or cfg.attention_sinks):
         raise ValueError(f"{cfg.name or cfg.family}: a sliding window and sinks are for the Llama / Mistral trunk")
     if cfg.attention_sinks and not cfg.sliding_window:

@@ -299,3 +299,14 @@ def test_an_adapter_keeps_the_attention_it_was_trained_with(tmp_path, monkeypatc
     assert gen.main(["--model", model, "--adapter", str(tmp_path / "older"), "--prompt", "a"]) == 0
     own = get_config(model)
     assert used.pop() == (own.sliding_window, own.attention_sinks)
+
+
+def test_full_causal_attention_of_a_model_with_sinks(tmp_path):
+    """A window of 0 takes the model's own sinks with it; sinks that are asked for still need a window."""
+    (tmp_path / "c.json").write_text(json.dumps(get_config("mistral-tiny", attention_sinks=4).to_hf_config()))
+    c = get_config(str(tmp_path / "c.json"), sliding_window=0)
+    assert (c.sliding_window, c.attention_sinks) == (0, 0)
+    c = get_config(str(tmp_path / "c.json"), sliding_window=30)
+    assert (c.sliding_window, c.attention_sinks) == (30, 4)
+    with pytest.raises(ValueError, match="needs a sliding window"):
+        get_config(str(tmp_path / "c.json"), sliding_window=0, attention_sinks=4)
