@@ -44,8 +44,6 @@ def generate(model, prompts: list[list[int]], max_new_tokens: int = 32, temperat
         raise ValueError(f"kv_bits must be 16 or 4, got {kv_bits}")
     if not hasattr(model, "layers") or not hasattr(model, "rope"):
         raise NotImplementedError("generate(): Llama / Mistral trunk models only")
-    was = model.training
-    model.eval()
     cfg = model.cfg
     dev = model.embed.device
     B = len(prompts)
@@ -57,6 +55,8 @@ def generate(model, prompts: list[list[int]], max_new_tokens: int = 32, temperat
     else:
         cache = ops.KVCache(len(model.layers), B, max_len, cfg.n_kv_heads, cfg.head_dim, dev, model.embed.dtype)
     gen = torch.Generator(device=dev).manual_seed(seed) if temperature > 0 else None
+    was = model.training
+    model.eval()
     try:
         # prefill, one prompt at a time (prompts differ in length)
         nxt = []

@@ -310,3 +310,12 @@ def test_full_causal_attention_of_a_model_with_sinks(tmp_path):
     assert (c.sliding_window, c.attention_sinks) == (30, 4)
     with pytest.raises(ValueError, match="needs a sliding window"):
         get_config(str(tmp_path / "c.json"), sliding_window=0, attention_sinks=4)
+
+
+@pytest.mark.parametrize("why", ["head_dim", "positions"])
+def test_a_refused_generation_leaves_the_model_in_its_mode(why):
+    m = build_model(get_config("llama-tiny"), None, device="cpu", dtype=torch.float32).train()  # head_dim 32, 512 positions
+    kw = dict(kv_bits=4) if why == "head_dim" else dict(max_new_tokens=600)
+    with pytest.raises(ValueError, match=why):
+        generate(m, [[5, 6]], **kw)
+    assert m.training
