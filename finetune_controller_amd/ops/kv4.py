@@ -81,6 +81,12 @@ def _maps(D: int):
     return (torch.stack(kb, 1), torch.tensor(kd), ks, torch.stack(vb, 1), torch.tensor(vd), vs)
 
 
+@functools.lru_cache(maxsize=None)
+def _maps_on(D: int, device: torch.device):
+    """``_maps`` on a device, copied there once: a captured step may copy nothing from the host."""
+    return tuple(z.to(device) for z in _maps(D))
+
+
 def quantize_reference(x: torch.Tensor):
     """``[..., D]`` -> (codes + 8 as uint8 ``[..., D]``, bf16 scales ``[..., D/32]``)."""
     g = x.float().unflatten(-1, (-1, KV4_GROUP))
@@ -99,24 +105,27 @@ def _held(codes: torch.Tensor, s: torch.Tensor) -> torch.Tensor:
     return ((codes.float() - 8.0).unflatten(-1, (-1, KV4_GROUP)) * s.float()[..., None]).flatten(-2)
 
 
-def _put(data: torch.Tensor, which: int, b, t, x: torch.Tensor, D: int):
-    """Quantise rows ``x`` [N, KV, D] into tokens (sequence b[i], position t[i])."""
-    m = [z.to(data.device) for z in _maps(D)]
+def _put(data: torch.Tensor, which: int, b, t, x: torch.Tensor, D: int, live):
+    """Quantise rows ``x`` [N, KV, D] into tokens (sequence b[i], position t[i]); where ``live`` is false the token's bytes
+    are written back as they were."""
+    m = _maps_on(D, data.device)
     by, d, sc = m[3 * which], m[3 * which + 1], m[3 * which + 2]
     codes, s = quantize_reference(x)
     bytes_ = codes[..., d[:, 0]] | (codes[..., d[:, 1]] << 4)
     sb = s.contiguous().view(torch.uint8).unflatten(-1, (-1, 2))
     tile, tt = t // KV4_TILE, t % KV4_TILE
     kv = torch.arange(x.shape[1], device=data.device)
-    bi, ki, ti = b[:, None, None], kv[None, :, None], tile[:, None, None]
-    data.index_put_((bi, ki, ti, by[tt][:, None]), bytes_)
+    bi, ki, ti, live = b[:, None, None], kv[None, :, None], tile[:, None, None], live[:, None, None]
+    at = (bi, ki, ti, by[tt][:, None])
+    data.index_put_(at, torch.where(live, bytes_, data[at]))
     for z in range(2):
-        data.index_put_((bi, ki, ti, sc[tt][:, None] + z), sb[..., z])
+        at = (bi, ki, ti, sc[tt][:, None] + z)
+        data.index_put_(at, torch.where(live, sb[..., z], data[at]))
 
 
 def _get(data: torch.Tensor, which: int, D: int) -> torch.Tensor:
     """fp32 values [B, KV, L, D] of a whole cache (L = its capacity)."""
-    m = [z.to(data.device) for z in _maps(D)]
+    m = _maps_on(D, data.device)
     by, d, sc = m[3 * which], m[3 * which + 1], m[3 * which + 2]
     B, KV, tiles, _ = data.shape
     raw = data[..., by.reshape(-1)].view(B, KV, tiles * KV4_TILE, -1)
@@ -165,14 +174,18 @@ def kv4_store(data: torch.Tensor, k: torch.Tensor, v: torch.Tensor, start: torch
     n = k.shape[1]
     if n == 0:
         return
-    i = torch.arange(n, device=data.device)
-    pos = start.long()[:, None] + i
-    ok = (pos >= 0) & (pos < cap)
+    # rows lo..hi - 1 of a sequence are written; the others are its nearest one of those once more (the same bytes again),
+    # so that nothing is read on the host
+    i, first = torch.arange(n, device=data.device), start.long()[:, None]
+    lo, hi = (-first).clamp(min=0), (cap - first).clamp(max=n)
     if count is not None:
-        ok &= i < count.long()[:, None]
-    b, r = ok.nonzero(as_tuple=True)
+        hi = torch.minimum(hi, count.long()[:, None])
+    live = hi > lo
+    r = torch.where(live, torch.minimum(torch.maximum(i, lo), hi - 1), torch.zeros_like(i))
+    t = (first + r).clamp(0, cap - 1).flatten()
+    b = torch.arange(B, device=data.device)[:, None].expand(B, n)
     for which, x in ((0, k), (1, v)):
-        _put(data, which, b, pos[b, r], x[b, r].unflatten(-1, (KV, D)), D)
+        _put(data, which, b.flatten(), t, x[b, r].flatten(0, 1).unflatten(-1, (KV, D)), D, live.expand(B, n).flatten())
 
 
 def kv4_load(data: torch.Tensor, start: torch.Tensor, n: int, D: int,

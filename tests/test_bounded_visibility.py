@@ -319,3 +319,14 @@ def test_a_refused_generation_leaves_the_model_in_its_mode(why):
     with pytest.raises(ValueError, match=why):
         generate(m, [[5, 6]], **kw)
     assert m.training
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (24, 3)])
+def test_gpu_generation_on_the_torch_path(bits, window, sinks, monkeypatch):
+    """FTC_KERNELS=torch: decode steps are captured by default there too, and a captured step equals an eager one."""
+    monkeypatch.setenv("FTC_KERNELS", "torch")
+    m = _model("cuda", torch.float32, sliding_window=window, attention_sinks=sinks)
+    eager = generate(m, _prompts(384), max_new_tokens=10, kv_bits=bits, graph=False)
+    assert generate(m, _prompts(384), max_new_tokens=10, kv_bits=bits) == eager

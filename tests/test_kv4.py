@@ -451,3 +451,22 @@ def test_decode_attention_has_no_derivative(dev, monkeypatch):
         with forward_ad.dual_level(), pytest.raises(NotImplementedError, match="derivative"):
             ops.decode_attention_kv4(forward_ad.make_dual(y, torch.ones_like(y)) * 2, data, lens, 32, 2, 1, 64)
     assert torch.equal(before, data)
+
+
+def test_the_torch_path_waits_for_nothing():
+    """Decode steps may be captured into a graph: no operation of theirs reads a tensor on the host."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class NoHostRead(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            assert func._overloadpacket not in (torch.ops.aten.nonzero, torch.ops.aten._local_scalar_dense,
+                                                torch.ops.aten.is_nonzero, torch.ops.aten.masked_select), func
+            return func(*args, **(kwargs or {}))
+
+    data = ops.kv4_alloc(3, 64, 2, 64)
+    qkv, lens = _rows(3, 8 * 64), torch.tensor([0, 5, 70], dtype=torch.int32)
+    k = _rows(3, 7, 2 * 64)
+    with NoHostRead():
+        ops.kv4_store(data, k, k, lens - 3, lens)
+        ops.kv4_load(data, lens, 4, 64)
+        ops.decode_attention_kv4(qkv, data, lens, 64, 4, 2, 64, window=9, sinks=2)
