@@ -705,11 +705,11 @@ inline void need_index(const at::Tensor& t, const at::Tensor& data, const char* 
              name, ": int32 [", data.size(0), "] on the cache's device, got ", t.scalar_type(), " ", t.sizes(), " on ",
              t.device());
 }
-// rows that cannot be read 16 bytes at a time are copied
-inline at::Tensor rows16(const at::Tensor& t) {
+// rows that cannot be read 16 bytes at a time are copied, the first `cols` (a multiple of 8) columns of them
+inline at::Tensor rows16(const at::Tensor& t, int64_t cols) {
   bool ok = t.stride(-1) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
   for (int64_t i = 0; i + 1 < t.dim(); ++i) ok = ok && (t.size(i) <= 1 || t.stride(i) % 8 == 0);
-  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+  return ok ? t : t.narrow(-1, 0, cols).clone(at::MemoryFormat::Contiguous);
 }
 
 void kv4_store_(at::Tensor& data, const at::Tensor& k_in, const at::Tensor& v_in, const at::Tensor& start,
@@ -729,7 +729,7 @@ void kv4_store_(at::Tensor& data, const at::Tensor& k_in, const at::Tensor& v_in
   need_value(n < (1LL << 30), "kv4_store: too many rows");
   if (n == 0) return;
   c10::DeviceGuard guard(data.device());
-  const at::Tensor k = rows16(k_in), v = rows16(v_in);
+  const at::Tensor k = rows16(k_in, KV * D), v = rows16(v_in, KV * D);
   check(ftc_kv4_store(data.data_ptr(), k.data_ptr(), v.data_ptr(), start.data_ptr<int>(),
                       count.has_value() ? count->data_ptr<int>() : nullptr, c.B, c.KV, (int)D, (int)n, c.tiles,
                       k.stride(0), k.stride(1), v.stride(0), v.stride(1), cur_stream()),
@@ -764,7 +764,7 @@ at::Tensor decode_attention_kv4(const at::Tensor& qkv_in, at::Tensor& data, cons
   need_value(sinks >= 0, "decode_attention_kv4: sinks must not be negative, got ", sinks);
   need_value(scale >= 0x1p-100 && scale <= 0x1p100, "decode_attention_kv4: scale must be positive and finite, got ", scale);
   c10::DeviceGuard guard(data.device());
-  const at::Tensor qkv = rows16(qkv_in);
+  const at::Tensor qkv = rows16(qkv_in, (H + 2 * KV) * D);
   auto out = empty_on(data, {c.B, H * D}, at::kBFloat16);
   const int win = (int)std::min<int64_t>(std::max<int64_t>(window, 0), 1 << 30);
   const int snk = (int)std::min<int64_t>(sinks, 1 << 30);

@@ -320,9 +320,11 @@ class _FlashPaddedTail(torch.autograd.Function):
         return dqkv, None, None, None, None, None, None, None, None, None, None, None
 
 
-def _rows16(t: torch.Tensor) -> torch.Tensor:
-    """``t`` itself if its rows can be read 16 bytes at a time, else a copy."""
-    if t.stride(1) == 1 and t.stride(0) >= t.shape[1] and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0:
+def _rows16(t: torch.Tensor, W: int) -> torch.Tensor:
+    """The first ``W`` (a multiple of 8) columns of ``t``: a view if its rows can be read 16 bytes at a time, else a copy."""
+    if t.shape[1] != W:
+        t = t[:, :W]
+    if t.stride(1) == 1 and t.stride(0) >= W and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -337,7 +339,7 @@ class _FlashSinks(torch.autograd.Function):
         Dp = kernel_head_dim(D)
         ctx.rope_grad = None
         if Dp == D:
-            x = _rows16(qkv)
+            x = _rows16(qkv, (H + 2 * KV) * D)
             o, olow, lse = ext().sink_fwd(x, B, S, H, KV, D, scale, window, sinks, out_pad, grad)
             out = o
             if rope_grad is not None and ROPE_BWD_FUSE and D == 128 and rope_grad.cos.shape[-1] == 64 and (
@@ -345,7 +347,7 @@ class _FlashSinks(torch.autograd.Function):
                 rope_grad.taken = True
                 ctx.rope_grad = rope_grad
         else:
-            x = _pad_heads(qkv, B, S, S, H + 2 * KV, D, Dp)
+            x = _pad_heads(qkv[:, :(H + 2 * KV) * D], B, S, S, H + 2 * KV, D, Dp)
             o, olow, lse = ext().sink_fwd(x, B, S, H, KV, Dp, scale, window, sinks, 0, grad)
             out = torch.empty(B * S, H * D + out_pad, dtype=qkv.dtype, device=qkv.device)[:, :H * D]
             _unpad_heads(o, out, B, S, S, H, D, Dp)
@@ -362,7 +364,7 @@ class _FlashSinks(torch.autograd.Function):
         nh = H + 2 * KV
         _gate_dw()
         if Dp == D:
-            do = _rows16(do)
+            do = _rows16(do, H * D)
             extra = W - nh * D  # qkv was wider than its heads: those columns get no gradient
             g = ext().sink_bwd(x, ctx.o, olow, do, lse, B, S, H, KV, D, scale, window, sinks, grad_pad if not extra else 0,
                                rg.cos if rg is not None else None, rg.sin if rg is not None else None,
@@ -408,7 +410,8 @@ def attention_packed(qkv: torch.Tensor, B: int, S: int, H: int, KV: int, D: int,
             raise ValueError(f"sinks: head_dim up to 128 in bf16, got {D}")
         # without derivatives: past autograd (a tangent goes to it, and is refused there)
         if kernel_head_dim(D) == D and not (qkv.requires_grad and torch.is_grad_enabled()) and not has_tangent(qkv):
-            return ext().sink_fwd(_rows16(qkv), B, S, H, KV, D, scale, int(window), int(sinks), out_pad, False)[0]
+            return ext().sink_fwd(_rows16(qkv, (H + 2 * KV) * D), B, S, H, KV, D, scale, int(window), int(sinks), out_pad,
+                                  False)[0]
         return _FlashSinks.apply(qkv, B, S, H, KV, D, int(window), int(sinks), scale, out_pad, grad_pad, rope_grad,
                                  torch.is_grad_enabled())
     if use_hip(qkv) and not sinks:

@@ -470,3 +470,15 @@ def test_the_torch_path_waits_for_nothing():
         ops.kv4_store(data, k, k, lens - 3, lens)
         ops.kv4_load(data, lens, 4, 64)
         ops.decode_attention_kv4(qkv, data, lens, 64, 4, 2, 64, window=9, sinks=2)
+
+
+@pytest.mark.gpu
+def test_decode_kernel_on_rows_of_odd_width():
+    """A contiguous projection of three more columns than the heads': its rows start off 16 bytes and are copied."""
+    B, H, KV, D, lens, cap = 3, 8, 2, 128, (40, 1, 64), 64
+    qkv, k, v = _decode_case(B, H, KV, D, lens, cap, seed=51)
+    data = ops.kv4_alloc(B, cap, KV, D, device="cuda")
+    ops.kv4_store(data, k.cuda(), v.cuda(), torch.zeros(B, dtype=torch.int32, device="cuda"))
+    wide = torch.cat([qkv, torch.full((B, 3), math.nan, dtype=BF)], 1).cuda()
+    got = ops.decode_attention_kv4(wide, data, torch.tensor(lens, dtype=torch.int32, device="cuda"), cap, H, KV, D)
+    _check(got, *_expected(qkv, k, v, lens, H, KV, D, D ** -0.5, 0, 0))

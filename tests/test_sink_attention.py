@@ -326,3 +326,35 @@ def test_forward_mode_is_refused(dev, D, grad, monkeypatch):
             ops.attention_packed(forward_ad.make_dual(x, torch.ones_like(x)), 1, 6, 2, 1, D, window=3, sinks=1)
         with forward_ad.dual_level(), torch.no_grad():  # the level alone refuses nothing
             assert ops.attention_packed(x, 1, 6, 2, 1, D, window=3, sinks=1).shape == (6, 2 * D)
+
+
+def _odd_rows(x, extra):
+    """``x`` in rows of ``extra`` more columns, contiguous: with an odd number of them most start off 16 bytes."""
+    return torch.cat([x, torch.full((x.shape[0], extra), math.nan, dtype=x.dtype, device=x.device)], 1)
+
+
+@pytest.mark.parametrize("extra", [0, 3, 8])
+def test_copied_rows_can_be_read_16_bytes_at_a_time(extra):
+    from finetune_controller_amd.ops.attention import _rows16
+
+    x = torch.randn(5, 256).to(BF)
+    for t in (_odd_rows(x, extra), _odd_rows(x, extra)[:, :256], _odd_rows(x, extra).t().contiguous().t()):
+        y = _rows16(t, 256)
+        assert torch.equal(y, x) and y.stride(1) == 1 and y.stride(0) % 8 == 0 and y.stride(0) >= 256
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("extra", [3, 8])
+@pytest.mark.parametrize("D", [64, 48])
+def test_more_columns_than_heads(extra, D):
+    B, S, H, KV, window, sinks = 1, 70, 2, 1, 9, 2
+    qkv, do = _inputs(B, S, H, KV, D, seed=10)
+    wo, to, wg, tg = _definition(qkv, do, B, S, H, KV, D, window, sinks, D ** -0.5)
+    x = _odd_rows(qkv, extra).cuda()
+    with torch.no_grad():
+        _close(ops.attention_packed(x, B, S, H, KV, D, window=window, sinks=sinks), wo, to)
+    o = ops.attention_packed(x.requires_grad_(), B, S, H, KV, D, window=window, sinks=sinks)
+    (g,) = torch.autograd.grad(o, x, do.cuda())
+    _close(o, wo, to)
+    _close(g[:, :qkv.shape[1]], wg, tg)
+    assert g.shape == x.shape and (g[:, qkv.shape[1]:] == 0).all()
