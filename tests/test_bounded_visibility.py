@@ -330,3 +330,32 @@ def test_gpu_generation_on_the_torch_path(bits, window, sinks, monkeypatch):
     m = _model("cuda", torch.float32, sliding_window=window, attention_sinks=sinks)
     eager = generate(m, _prompts(384), max_new_tokens=10, kv_bits=bits, graph=False)
     assert generate(m, _prompts(384), max_new_tokens=10, kv_bits=bits) == eager
+
+
+@pytest.mark.gpu
+def test_allocations_are_seen_by_dispatch_modes():
+    """A mode that follows allocations (a memory tracker) sees what the operators return."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Allocated(TorchDispatchMode):
+        def __init__(self):
+            super().__init__()
+            self.at = set()
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            out = func(*args, **(kwargs or {}))
+            if isinstance(out, torch.Tensor) and "empty" in str(func):
+                self.at.add(out.untyped_storage().data_ptr())
+            return out
+
+    H, KV, D, n = 2, 1, 64, 40
+    bf, i32 = dict(dtype=torch.bfloat16, device="cuda"), dict(dtype=torch.int32, device="cuda")
+    x = torch.randn(n, (H + 2 * KV) * D, **bf).requires_grad_()
+    data, start = ops.kv4_alloc(1, 64, KV, D, device="cuda"), torch.zeros(1, **i32)
+    with Allocated() as seen:
+        o = ops.attention_packed(x, 1, n, H, KV, D, window=9, sinks=2)
+        (g,) = torch.autograd.grad(o, x, torch.ones_like(o))
+        alone = ops.attention_packed(x.detach(), 1, n, H, KV, D, window=9, sinks=2)
+        rows = ops.kv4_load(data, start, 5, D)
+        new = ops.decode_attention_kv4(x.detach()[:1], data, start + 1, 64, H, KV, D)
+    assert [t.untyped_storage().data_ptr() in seen.at for t in (o, g, alone, *rows, new)] == [True] * 6
