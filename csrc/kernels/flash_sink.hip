@@ -104,7 +104,6 @@ __global__ __launch_bounds__(64 * WAVES * GR, 8 / WAVES) void sink_fwd_kernel(Fw
   const int q0 = qb * BQ;
   const int qrow = q0 + wave * 32 + lr;
   const bool qvalid = qrow < S;
-  static_assert(BQ == 32 * WAVES, "geometry");
 
   bf16x8 qf[DSTEPS];
   auto load_q = [&]() __attribute__((always_inline)) {
@@ -365,41 +364,28 @@ __global__ __launch_bounds__(64 * WAVES * GR, 8 / WAVES) void sink_fwd_kernel(Fw
       if (qvalid) *reinterpret_cast<uint4*>(lp + dt * 32 + 16 * hh) = make_uint4(a0[0], a0[1], b0[0], b0[1]);
     }
   }
-  if ((a.o_rs & 7) == 0) {
-    // 16-byte stores (the store tail is issue-bound): lanes l and l ^ 32 hold the same
-    // query row, d runs {8 g4 + 4 hh + 0..3}; two v_permlane32_swap per dword pair give lane half hh
-    // the 16 contiguous d [16 hh, 16 hh + 16) of each 32-wide tile -> 2 x dwordx4 instead of 4 x dwordx2
+  // 16-byte stores (the store tail is issue-bound): lanes l and l ^ 32 hold the same
+  // query row, d runs {8 g4 + 4 hh + 0..3}; two v_permlane32_swap per dword pair give lane half hh
+  // the 16 contiguous d [16 hh, 16 hh + 16) of each 32-wide tile -> 2 x dwordx4 instead of 4 x dwordx2
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) {
-      uint32_t w[4][2];
+  for (int dt = 0; dt < DT; ++dt) {
+    uint32_t w[4][2];
 #pragma unroll
-      for (int g4 = 0; g4 < 4; ++g4) {
-        w[g4][0] = pack_bf2(o[dt][4 * g4 + 0] * inv, o[dt][4 * g4 + 1] * inv);
-        w[g4][1] = pack_bf2(o[dt][4 * g4 + 2] * inv, o[dt][4 * g4 + 3] * inv);
-      }
-      // swap(x, y): lanes 0-31 keep x and receive the upper half's x; lanes 32-63 receive the lower
-      // half's y and keep y -> (x_own | x_partner) below, (y_partner | y_own) above
-      const auto a0 = __builtin_amdgcn_permlane32_swap(w[0][0], w[2][0], false, false);
-      const auto a1 = __builtin_amdgcn_permlane32_swap(w[0][1], w[2][1], false, false);
-      const auto b0 = __builtin_amdgcn_permlane32_swap(w[1][0], w[3][0], false, false);
-      const auto b1 = __builtin_amdgcn_permlane32_swap(w[1][1], w[3][1], false, false);
-      if (qvalid) {
-        const int d = dt * 32 + 16 * hh;
-        *reinterpret_cast<uint4*>(op + d) = make_uint4(a0[0], a1[0], a0[1], a1[1]);
-        *reinterpret_cast<uint4*>(op + d + 8) = make_uint4(b0[0], b1[0], b0[1], b1[1]);
-      }
+    for (int g4 = 0; g4 < 4; ++g4) {
+      w[g4][0] = pack_bf2(o[dt][4 * g4 + 0] * inv, o[dt][4 * g4 + 1] * inv);
+      w[g4][1] = pack_bf2(o[dt][4 * g4 + 2] * inv, o[dt][4 * g4 + 3] * inv);
     }
-  } else if (qvalid) {
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-      for (int g4 = 0; g4 < 4; ++g4) {
-        const int d = dt * 32 + 8 * g4 + 4 * hh;
-        uint2 w;
-        w.x = pack_bf2(o[dt][4 * g4 + 0] * inv, o[dt][4 * g4 + 1] * inv);
-        w.y = pack_bf2(o[dt][4 * g4 + 2] * inv, o[dt][4 * g4 + 3] * inv);
-        *reinterpret_cast<uint2*>(op + d) = w;
-      }
+    // swap(x, y): lanes 0-31 keep x and receive the upper half's x; lanes 32-63 receive the lower
+    // half's y and keep y -> (x_own | x_partner) below, (y_partner | y_own) above
+    const auto a0 = __builtin_amdgcn_permlane32_swap(w[0][0], w[2][0], false, false);
+    const auto a1 = __builtin_amdgcn_permlane32_swap(w[0][1], w[2][1], false, false);
+    const auto b0 = __builtin_amdgcn_permlane32_swap(w[1][0], w[3][0], false, false);
+    const auto b1 = __builtin_amdgcn_permlane32_swap(w[1][1], w[3][1], false, false);
+    if (qvalid) {
+      const int d = dt * 32 + 16 * hh;
+      *reinterpret_cast<uint4*>(op + d) = make_uint4(a0[0], a1[0], a0[1], a1[1]);
+      *reinterpret_cast<uint4*>(op + d + 8) = make_uint4(b0[0], b1[0], b0[1], b1[1]);
+    }
   }
   if constexpr (GRAD) {
     const float ltot = l + __shfl_xor(l, 32, 64);
@@ -442,7 +428,7 @@ __global__ __launch_bounds__(512, 1) void sink_dkdv_kernel(BwdArgs a) {
   constexpr int WAVES = 8, NT = 64 * WAVES;
   constexpr int KBYTES = BKV * D * 2, QBYTES = BQ2 * D * 2;
   constexpr int SLICE = 2 * QBYTES + 2 * BQ2 * 4;  // Q | dO | -lse/scale | -delta
-  // K and the three ring slots are DISTINCT __shared__ objects: the compiler then knows (LDS alias
+  // K and the five ring slots are DISTINCT __shared__ objects: the compiler then knows (LDS alias
   // scopes) that reading one slot does not depend on the DMA still writing the others, instead of
   // draining every DMA (vmcnt(0)) before the first ds_read of each slice
   __shared__ __attribute__((aligned(16))) char Ks[KBYTES];
@@ -659,7 +645,7 @@ __global__ __launch_bounds__(512, 1) void sink_dkdv_kernel(BwdArgs a) {
     const int qt = qbeg + ((it0 + it) % nqt) * BQ2;
     return qt + BQ2 - 1 >= wkey0 && qt - (wkey0 + 31) < a.window;
   };
-  // one barrier per slice: slice it is in LDS for every wave, the DMA of slice it + 2 goes out
+  // one barrier per slice: slice it is in LDS for every wave, the DMA of slice it + DIST goes out
   auto sync_slice = [&](const int it, char* dma_slot) __attribute__((always_inline)) {
     if (it + 2 < total) {
       __builtin_amdgcn_s_waitcnt(VM_TWO);  // slices it+1, it+2 may fly on
@@ -746,12 +732,11 @@ __global__ __launch_bounds__(512, 1) void sink_dkdv_kernel(BwdArgs a) {
   }
   uint16_t* dkp = a.dk + ((long long)b * S + key) * a.dkv_rs + (long long)kvh * D;
   uint16_t* dvp = a.dv + ((long long)b * S + key) * a.dkv_rs + (long long)kvh * D;
-  const bool wide = (a.dkv_rs & 7) == 0;
   if constexpr (D == 128) {
     if (a.rcos) rope_inv_rows<DT>(dk, a, (long long)b * S + key, hh);
   }
-  store_rows<DT>(dkp, dk, a.scale, hh, wide);
-  store_rows<DT>(dvp, dv, 1.0f, hh, wide);
+  store_rows<DT>(dkp, dk, a.scale, hh, true);
+  store_rows<DT>(dvp, dv, 1.0f, hh, true);
 }
 
 // dK / dV rows of key blocks that were swept in parts: the parts' sums and the sink keys' far sums in order, then the
@@ -1125,7 +1110,7 @@ __global__ __launch_bounds__(256, 2) void sink_dq_kernel(BwdArgs a) {
   if constexpr (D == 128) {
     if (a.rcos) rope_inv_rows<DT>(dq, a, (long long)b * S + qrow, hh);
   }
-  store_rows<DT>(op, dq, a.scale, hh, (a.dq_rs & 7) == 0);
+  store_rows<DT>(op, dq, a.scale, hh, true);
 }
 
 template <int D, bool GRAD>
@@ -1139,9 +1124,9 @@ void launch_fwd(const FwdArgs& a, long long blocks, bool two, hipStream_t stream
 extern "C" int ftc_sink_fwd(const void* q, const void* k, const void* v, void* o, void* olow, float* lse, int B, int S, int H, int KV,
                             int D, long long q_rs, long long kv_rs, long long o_rs, float scale, int window, int sinks,
                             hipStream_t stream) {
-  // the rows of one (batch, kv head) are addressed with 32-bit buffer offsets
+  // the rows of one (batch, kv head) are addressed with 32-bit buffer offsets; every row starts on 16 bytes
   if (B < 1 || S < 1 || KV < 1 || H % KV != 0 || (D != 128 && D != 64) || window < 1 || sinks < 0 ||
-      (long long)S * kv_rs * 2 >= (1LL << 31))
+      ((q_rs | kv_rs | o_rs) & 7) || (long long)S * kv_rs * 2 >= (1LL << 31))
     return -1;
   const int BQ = 32 * WAVES;
   FwdArgs a{(const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, (uint16_t*)o, (uint8_t*)olow, lse, q_rs,
@@ -1206,6 +1191,7 @@ extern "C" int ftc_sink_bwd(const void* q, const void* k, const void* v, const v
                             long long dkv_rs, float scale, int window, int sinks, const float* rope_cos,
                             const float* rope_sin, const int* rope_pos, hipStream_t stream) {
   if (B < 1 || S < 1 || KV < 1 || H % KV != 0 || (D != 128 && D != 64) || window < 1 || sinks < 0) return -1;
+  if ((q_rs | kv_rs | o_rs | do_rs | dq_rs | dkv_rs) & 7) return -1;  // every row starts on 16 bytes
   if (rope_cos && (D != 128 || !rope_sin || ((reinterpret_cast<uintptr_t>(rope_cos) |
                                                reinterpret_cast<uintptr_t>(rope_sin)) & 15)))
     return -1;

@@ -418,3 +418,20 @@ def test_the_backward_reads_the_low_byte(B, S, H, KV, D, window, sinks):
     rounded = (D ** -0.5 * off * k).flatten()
     got = g[:, :H * D].double().cpu().flatten()
     assert got.norm() < 0.5 * rounded.norm(), float(got.norm() / rounded.norm())
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the launchers' own checks, called without tensors")
+def test_launchers_refuse_rows_off_16_bytes():
+    """The kernels load and store 16 bytes at a time: any row stride that is no multiple of 8 is refused before a launch."""
+    import ctypes
+
+    from finetune_controller_amd.ops._backend import load_ext
+
+    lib = ctypes.CDLL(load_ext().__file__)
+    null, i, ll, f = ctypes.c_void_p(), ctypes.c_int, ctypes.c_longlong, ctypes.c_float
+    for odd in range(3):
+        rs = [ll(256 + (4 if j == odd else 0)) for j in range(3)]
+        assert lib.ftc_sink_fwd(*[null] * 6, i(1), i(8), i(2), i(1), i(64), *rs, f(0.1), i(4), i(1), null) == -1
+    for odd in range(6):
+        rs = [ll(256 + (4 if j == odd else 0)) for j in range(6)]
+        assert lib.ftc_sink_bwd(*[null] * 11, i(1), i(8), i(2), i(1), i(64), *rs, f(0.1), i(4), i(1), *[null] * 4) == -1
