@@ -26,6 +26,7 @@ import os
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 _lock = threading.Lock()
 _ext = None
@@ -80,8 +81,9 @@ def ext():
 
 
 def has_tangent(t: torch.Tensor) -> bool:
-    """``t`` carries a forward-mode derivative (``torch.autograd.forward_ad``), with or without ``requires_grad``."""
-    return torch.autograd.forward_ad.unpack_dual(t).tangent is not None
+    """``t`` carries a forward-mode derivative, with or without ``requires_grad``.  Outside every ``dual_level`` no tensor
+    does: that alone is looked at there (0.1 us; unpacking takes 0.5, where a small call takes 3 to 6)."""
+    return getattr(forward_ad, "_current_level", 0) >= 0 and forward_ad.unpack_dual(t).tangent is not None
 
 
 def stream_ptr(device: torch.device | None = None) -> int:
