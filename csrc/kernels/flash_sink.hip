@@ -1133,8 +1133,8 @@ extern "C" int ftc_sink_fwd(const void* q, const void* k, const void* v, void* o
             kv_rs, o_rs, B, S, H, KV, (S + BQ - 1) / BQ, scale * LOG2E, window < S ? window : S, sinks < S ? sinks : S};
   const long long blocks = (long long)a.nqb * B * H;
   if (blocks > 0x7fffffffLL) return -1;
-  // One group where the blocks fill the chip, two where each has a CU to itself and more than two tiles (one group, two
-  // groups, us): 1 x 1000 tokens, 32 / 8 heads x 128 (256 blocks), window 999: 23.5, 19.9; 512: 20.1, 18.3; 16: 11.8, 11.7;
+  // One group where the blocks fill the chip, two where each has a CU to itself and the sequence is longer than a block (in
+  // one block of queries there are at most two tiles to share) (one group, two groups, us): 1 x 1000 tokens, 32 / 8 heads x 128 (256 blocks), window 999: 23.5, 19.9; 512: 20.1, 18.3; 16: 11.8, 11.7;
   // 1 x 1001, 8 / 2 heads, window 256 (64 blocks): 15.0, 14.4; 320 blocks, window 512: 21.6, 21.5; 512 blocks: 35.7, 42.8;
   // 1 x 100, 8 heads: 6.8, 7.7.
   const bool two = blocks <= 256 && S > BQ;

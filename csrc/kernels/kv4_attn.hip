@@ -444,7 +444,8 @@ Plan kv4_plan(int B, int H, int KV, int D, int max_len, int window, int sinks) {
   // tokens, 512 items: 8.9 us with 4 waves, 11.5 with 8).
   p.nw = items > 256 && vis < 32 ? 4 : 8;
   // Parts: the number that a model of the launch finds quickest -- rounds of 256 workgroups, 1.8 us a record and
-  // wave (the cache bytes at 5.2 TB/s) plus 2.5 us a workgroup, and 3 us for the join.  Measured against every
+  // wave plus 2.5 us a workgroup, and 3 us for the join.  The 1.8 us are a record's latency: a wave takes 1.5 to 1.8
+  // whether 8 CUs are busy or all (192 us for 128 records a wave on 8); with all of them busy that is 5.2 TB/s as well.  Measured against every
   // split from 1 to 128: it picks the quickest or one within 4 % (one 32768-token sequence, 8 items: 32 parts
   // 15.0 us, 24 parts 16.4, unsplit 192; 16 sequences at a 4096 window: 2 parts 18.9, 1 part 30.9; 32 x 4096
   // tokens: unsplit 25.3, 2 parts 30.0).

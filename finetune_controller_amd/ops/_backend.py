@@ -82,7 +82,7 @@ def ext():
 
 def has_tangent(t: torch.Tensor) -> bool:
     """``t`` carries a forward-mode derivative, with or without ``requires_grad``.  Outside every ``dual_level`` no tensor
-    does: that alone is looked at there (0.1 us; unpacking takes 0.5, where a small call takes 3 to 6)."""
+    does: that alone is looked at there (0.2 us of the host, unpacking takes 0.5)."""
     return getattr(forward_ad, "_current_level", 0) >= 0 and forward_ad.unpack_dual(t).tangent is not None
 
 
