@@ -10,8 +10,9 @@
 //     otherwise sweep the whole sequence while the others sweep a window.
 // No float atomics: results do not depend on the order of workgroups.
 // Bound: MFMA with the softmax's VALU in the same waves.  32 / 8 heads x 128, 4 sinks: forward of 16384 tokens, window
-// 4096: 912 us, 1056 TF/s (MFMA busy 0.55); 4 x 4096, window 1024: forward 314 us, dQ 427, dK / dV 600, far queries 55
-// (MFMA busy 0.38, 0.48, 0.36: blocks of 128 queries or 256 keys reach past a window of 1024 by 12 or 18 %).
+// 4096: 912 to 956 us on different cards, 1007 to 1056 TF/s (MFMA busy 0.55); 4 x 4096, window 1024: forward 314 to 323 us,
+// dQ 427 to 434, dK / dV 600 to 613, far queries 55 (MFMA busy 0.38, 0.48, 0.36: blocks of 128 queries or 256 keys reach
+// past a window of 1024 by 12 or 18 %, and dK / dV's workgroups fill two rounds unevenly).
 #include "flash_tiles.h"
 
 using namespace ftc;
