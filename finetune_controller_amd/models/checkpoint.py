@@ -95,9 +95,10 @@ def adapter_attention(path: str) -> tuple[int, int]:
         if os.path.exists(f):
             with open(f) as h:
                 rec = json.load(h)
-            rec = rec.get("model", {}) if name != ADAPTER_ATTENTION else rec
-            if "sliding_window" in rec:
-                return int(rec["sliding_window"]), int(rec.get("attention_sinks", 0))
+            if name != ADAPTER_ATTENTION:
+                rec = rec.get("model") if isinstance(rec, dict) else None
+            if isinstance(rec, dict) and isinstance(rec.get("sliding_window"), int):
+                return rec["sliding_window"], int(rec.get("attention_sinks") or 0)
     return -1, -1
 
 

@@ -359,3 +359,11 @@ def test_allocations_are_seen_by_dispatch_modes():
         rows = ops.kv4_load(data, start, 5, D)
         new = ops.decode_attention_kv4(x.detach()[:1], data, start + 1, 64, H, KV, D)
     assert [t.untyped_storage().data_ptr() in seen.at for t in (o, g, alone, *rows, new)] == [True] * 6
+
+
+@pytest.mark.parametrize("record", [{"model": "some/base"}, [1], {"model": {"sliding_window": None}}, {}])
+def test_records_of_other_tools_say_nothing_of_the_attention(tmp_path, record):
+    from finetune_controller_amd.models.checkpoint import adapter_attention
+
+    (tmp_path / "training_config.json").write_text(json.dumps(record))
+    assert adapter_attention(str(tmp_path)) == (-1, -1)
